@@ -90,7 +90,9 @@ wg_status wg_device_set_stream(wg_device *dev, void *stream);
 /* Waits until the handle's stream is idle. */
 wg_status wg_device_sync(wg_device *dev);
 /* Waits, then reports (and clears) a device-side error word: WG_ERR_KERNEL_TIMEOUT
- * when a kernel's bounded wait gave up since the last check. */
+ * when a kernel's bounded wait gave up since the last check, else
+ * WG_ERR_INVALID_ARGUMENT when a grouped product found offsets (read on the
+ * device) that decrease or leave its rows. */
 wg_status wg_device_check(wg_device *dev);
 /* Failure-detection self-test (no counterpart in the reference). Queues one
  * CTA that waits, with the same clock-bounded mbarrier wait the tensor-core
@@ -378,6 +380,45 @@ wg_status wg_sgemv_dev(wg_device *dev, int trans, int64_t m, int64_t n, float al
                        const float *x, int64_t incx, float beta, float *y, int64_t incy);
 wg_status wg_dgemv_dev(wg_device *dev, int trans, int64_t m, int64_t n, double alpha, const double *A, int64_t lda,
                        const double *x, int64_t incx, double beta, double *y, int64_t incy);
+
+/* ---- products grouped by expert (no counterpart in the reference) ---------
+ * Layers that route each row to one of several weight matrices. Row-major
+ * matrices here (the layout of such layers, and wgblas's default), 16-bit
+ * operands, sums in 32 bits on the tensor cores, one rounding to C's type.
+ *
+ * `offsets` points at groups + 1 int32 on the device: rows offsets[g] up to
+ * offsets[g + 1] belong to group g; they are read when the kernel runs, so a
+ * router's output needs no copy to the host. A group may have no rows. Rows
+ * before offsets[0] and from offsets[groups] on belong to no group and are left
+ * as they are in C. Offsets that decrease or leave [0, rows] are clamped (each
+ * to the range and to the largest before it) and reported by wg_device_check.
+ *
+ * alpha, beta as for wg_sgemm: alpha == 0 reads neither A nor B, beta == 0 does
+ * not read C. C must not overlap A or B. Pointers, leading dimensions and
+ * strides need only the alignment of their elements; operands whose bases are
+ * 16-byte aligned and whose rows (and strideB) are whole 16-byte units load by
+ * TMA. Queued on the device stream; no workspace. gpu_ms as for wg_sgemm. */
+#define WG_TYPE_F32 0
+#define WG_TYPE_BF16 1
+#define WG_TYPE_F16 2
+#define WG_MAX_GROUPS 1024
+/* Rows form: C[r] = alpha * A[r] op(B_g) + beta * C[r] for the rows r of group
+ * g. A is m x k (lda >= k), C is m x n (ldc >= n); B_g = B + g * strideB is
+ * stored k x n (transB 0, ldb >= n) or n x k (transB 1, ldb >= k); strideB 0
+ * shares one matrix. type: A and B, WG_TYPE_BF16 or WG_TYPE_F16; ctype: the same
+ * or WG_TYPE_F32. With the weights stored n x k, transB 1 is a layer's forward
+ * product and transB 0 (n and k exchanged) the gradient of its input. */
+wg_status wg_gemm_grouped_dev(wg_device *dev, int type, int ctype, int transB, int64_t groups, int64_t m, int64_t n,
+                              int64_t k, float alpha, const void *A, int64_t lda, const void *B, int64_t ldb,
+                              int64_t strideB, const int *offsets, float beta, void *C, int64_t ldc, float *gpu_ms);
+/* Inner form: C_g = alpha * A[rows of g]^T B[rows of g] + beta * C_g. A is k x m
+ * (lda >= m), B is k x n (ldb >= n), the k rows are grouped by offsets;
+ * C_g = C + g * strideC is m x n (ldc >= n). A group without rows gives
+ * beta * C_g (zeros when beta is 0). The gradient of the weights. */
+wg_status wg_gemm_grouped_inner_dev(wg_device *dev, int type, int ctype, int64_t groups, int64_t m, int64_t n,
+                                    int64_t k, float alpha, const void *A, int64_t lda, const void *B, int64_t ldb,
+                                    const int *offsets, float beta, void *C, int64_t ldc, int64_t strideC,
+                                    float *gpu_ms);
 
 /* ---- multi-GPU: C sharded by row blocks, B broadcast over NVLink (NCCL) ---- */
 /* The reference drives several GPUs only as independent devices with no data

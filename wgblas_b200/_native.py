@@ -157,6 +157,13 @@ _sig("wg_sgemv_dev", _st, *_gemv_dims, ct.c_float, ct.c_void_p, _i64, ct.c_void_
      _i64)
 _sig("wg_dgemv_dev", _st, *_gemv_dims, ct.c_double, ct.c_void_p, _i64, ct.c_void_p, _i64, ct.c_double, ct.c_void_p,
      _i64)
+WG_TYPE_F32, WG_TYPE_BF16, WG_TYPE_F16 = 0, 1, 2
+WG_MAX_GROUPS = 1024
+_ptr = ct.c_void_p
+_sig("wg_gemm_grouped_dev", _st, c_dev_p, ct.c_int, ct.c_int, ct.c_int, _i64, _i64, _i64, _i64, ct.c_float, _ptr, _i64,
+     _ptr, _i64, _i64, _ptr, ct.c_float, _ptr, _i64, _f32p)
+_sig("wg_gemm_grouped_inner_dev", _st, c_dev_p, ct.c_int, ct.c_int, _i64, _i64, _i64, _i64, ct.c_float, _ptr, _i64,
+     _ptr, _i64, _ptr, ct.c_float, _ptr, _i64, _i64, _f32p)
 c_comm_p = ct.c_void_p
 _sig("wg_comm_unique_id", _st, ct.c_char_p, ct.c_size_t)
 _sig("wg_comm_init_rank", _st, c_dev_p, ct.c_int, ct.c_int, ct.c_char_p, ct.c_size_t, ct.c_int, ct.POINTER(c_comm_p))

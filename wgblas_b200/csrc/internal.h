@@ -67,7 +67,8 @@ enum {
   WG_DERR_MMA_WAIT = 2u,  // the epilogue gave up waiting for the accumulator
   WG_DERR_TMEM = 4u,      // TMEM allocation returned an unusable address
   WG_DERR_SELFTEST = 8u,  // wg_selftest_bounded_wait's wait ran out, as it is meant to
-  WG_DERR_FLOW_WAIT = 16u  // a strsm flow CTA gave up waiting for an earlier block
+  WG_DERR_FLOW_WAIT = 16u,  // a strsm flow CTA gave up waiting for an earlier block
+  WG_DERR_OFFSETS = 32u     // a grouped product's offsets decreased or left its rows (not a wait)
 };
 
 struct wg_device {

@@ -183,6 +183,9 @@ extern "C" wg_status wg_device_check(wg_device *d) {
   if (word) {
     WG_CUDA(cudaMemsetAsync(d->dwords + WG_DW_ERROR, 0, sizeof(unsigned), d->stream));
     WG_CUDA(cudaStreamSynchronize(d->stream));
+    if (word == WG_DERR_OFFSETS)
+      return wg_fail(WG_ERR_INVALID_ARGUMENT,
+                     "offsets of a grouped product decreased or left its rows; they were clamped");
     return wg_fail(WG_ERR_KERNEL_TIMEOUT,
                    "a kernel's bounded wait gave up (device error word 0x%x); its output "
                    "is incomplete", word);
