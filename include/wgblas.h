@@ -420,6 +420,45 @@ wg_status wg_gemm_grouped_inner_dev(wg_device *dev, int type, int ctype, int64_t
                                     const int *offsets, float beta, void *C, int64_t ldc, int64_t strideC,
                                     float *gpu_ms);
 
+/* ---- microscaled 4-bit floating point (no counterpart in the reference) ----
+ * OCP MXFP4. 32 neighbouring elements of a row share a scale 2^e, stored as the
+ * byte e + 127 (255: NaN); an element is one of 0, .5, 1, 1.5, 2, 3, 4, 6 or its
+ * negative. A quantised rows x cols matrix is two arrays, both 16-byte aligned:
+ *   codes   two elements a byte (the even column in the low half); a row is
+ *           ceil(cols / 32) * 16 bytes, padding elements zero;
+ *   scales  tiles of 128 rows x 4 blocks, 512 bytes each, ceil(cols / 128) tiles
+ *           a tile row; row r, block b of a tile at 16 * (r % 32) + 4 * (r / 32) + b;
+ *           padding bytes zero.
+ * A batch of matrices is stored one after the other in both. A matrix whose rows
+ * are grouped (offsets as above) begins each group's scales at a new tile row,
+ * so its scales have up to ceil(rows / 128) + groups tile rows; its codes are as
+ * ever. All calls are queued on the device stream; gpu_ms as for wg_sgemm.
+ *
+ * Quantises op(X), rows x cols (X stored rows x cols, or cols x rows when trans;
+ * type WG_TYPE_F32, _BF16 or _F16; batch matrices strideX apart): for each block
+ * e = max(floor(log2(max |x|)) - 2, -127), elements x / 2^e rounded to nearest,
+ * ties to even, what exceeds 6 to 6; a block with a NaN or infinity gets the
+ * scale 255. groups > 0 (with offsets, batch 1, trans 0): rows of no group are
+ * not written. */
+wg_status wg_mx_quantize_dev(wg_device *dev, int type, int trans, int64_t batch, int64_t rows, int64_t cols,
+                             const void *X, int64_t ldx, int64_t strideX, int64_t groups, const int *offsets,
+                             void *codes, void *scales, float *gpu_ms);
+/* X (rows x cols, ldx, batch matrices strideX apart) := the values the codes stand for, rounded to X's type. */
+wg_status wg_mx_dequantize_dev(wg_device *dev, int type, int64_t batch, int64_t rows, int64_t cols, const void *codes,
+                               const void *scales, int64_t groups, const int *offsets, void *X, int64_t ldx,
+                               int64_t strideX, float *gpu_ms);
+/* C (m x n row-major, ldc, WG_TYPE_F32, _BF16 or _F16) = alpha * A B^T + beta * C,
+ * A m x k and B n x k quantised along k; sums in 32 bits, one rounding. */
+wg_status wg_mx_gemm_dev(wg_device *dev, int ctype, int64_t m, int64_t n, int64_t k, float alpha, const void *A,
+                         const void *A_scales, const void *B, const void *B_scales, float beta, void *C, int64_t ldc,
+                         float *gpu_ms);
+/* C[r] = alpha * A[r] B_g^T + beta * C[r] for the rows r of group g: A m x k with
+ * grouped rows, B a batch of `groups` n x k matrices. Rows of no group keep their C. */
+wg_status wg_mx_gemm_grouped_dev(wg_device *dev, int ctype, int64_t groups, int64_t m, int64_t n, int64_t k,
+                                 float alpha, const void *A, const void *A_scales, const void *B,
+                                 const void *B_scales, const int *offsets, float beta, void *C, int64_t ldc,
+                                 float *gpu_ms);
+
 /* ---- multi-GPU: C sharded by row blocks, B broadcast over NVLink (NCCL) ---- */
 /* The reference drives several GPUs only as independent devices with no data
  * exchange (src/init.mjs:14-29, examples/init-two-gpus/init-two-gpus.js); this

@@ -18,6 +18,8 @@ from .gemmtr import dgemmtr, dsyr2k, dsyrk, sgemmtr, ssyr2k, ssyrk  # noqa: F401
 from .gemv import dgemv, sgemv  # noqa: F401
 from .grouped import gemmGrouped, gemmGroupedInner  # noqa: F401
 from .level3 import dsymm, dtrmm, ssymm, strmm, strsm  # noqa: F401
+from .mx import (GpuMxMatrix, mxCodesSize, mxDecode, mxDequantize, mxGemm, mxGemmGrouped,  # noqa: F401
+                 mxQuantize, mxScalesSize)
 from .random import (fill_uniform, randomFloat32Array, randomFloat64Array,  # noqa: F401
                      randomNormalFloat32Array, randomNormalFloat64Array)
 
@@ -27,6 +29,7 @@ __all__ = [
     "sgemm", "dgemm", "sgemmtr", "dgemmtr", "ssyrk", "dsyrk", "ssyr2k", "dsyr2k",
     "ssymm", "dsymm", "strmm", "dtrmm", "strsm", "sgemv", "dgemv",
     "GpuArray", "toBfloat16", "fromBfloat16", "gemmGrouped", "gemmGroupedInner",
+    "GpuMxMatrix", "mxCodesSize", "mxScalesSize", "mxDecode", "mxQuantize", "mxDequantize", "mxGemm", "mxGemmGrouped",
     "randomFloat32Array", "randomFloat64Array",
     "randomNormalFloat32Array", "randomNormalFloat64Array", "fill_uniform",
 ]

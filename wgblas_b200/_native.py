@@ -164,6 +164,13 @@ _sig("wg_gemm_grouped_dev", _st, c_dev_p, ct.c_int, ct.c_int, ct.c_int, _i64, _i
      _ptr, _i64, _i64, _ptr, ct.c_float, _ptr, _i64, _f32p)
 _sig("wg_gemm_grouped_inner_dev", _st, c_dev_p, ct.c_int, ct.c_int, _i64, _i64, _i64, _i64, ct.c_float, _ptr, _i64,
      _ptr, _i64, _ptr, ct.c_float, _ptr, _i64, _i64, _f32p)
+_sig("wg_mx_quantize_dev", _st, c_dev_p, ct.c_int, ct.c_int, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr,
+     _f32p)
+_sig("wg_mx_dequantize_dev", _st, c_dev_p, ct.c_int, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _i64, _f32p)
+_sig("wg_mx_gemm_dev", _st, c_dev_p, ct.c_int, _i64, _i64, _i64, ct.c_float, _ptr, _ptr, _ptr, _ptr, ct.c_float, _ptr,
+     _i64, _f32p)
+_sig("wg_mx_gemm_grouped_dev", _st, c_dev_p, ct.c_int, _i64, _i64, _i64, _i64, ct.c_float, _ptr, _ptr, _ptr, _ptr, _ptr,
+     ct.c_float, _ptr, _i64, _f32p)
 c_comm_p = ct.c_void_p
 _sig("wg_comm_unique_id", _st, ct.c_char_p, ct.c_size_t)
 _sig("wg_comm_init_rank", _st, c_dev_p, ct.c_int, ct.c_int, ct.c_char_p, ct.c_size_t, ct.c_int, ct.POINTER(c_comm_p))

@@ -18,6 +18,7 @@
 namespace {
 
 using wgg::BL;
+using wgg::mbar_arrive;
 using wgg::WAIT_BUDGET;
 
 constexpr int BK = 64;          // k-block: 64 16-bit elements, one 128-byte swizzle span
@@ -94,10 +95,6 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(wgtc::smem_addr(bar)) : "memory");
 }
 
 // One output tile: lanes [l0, l0 + 128) and columns [n0, n0 + nv) of group g,

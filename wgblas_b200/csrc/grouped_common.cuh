@@ -30,11 +30,12 @@ constexpr long long WAIT_BUDGET = 4000000000LL;  // SM clocks (~2 s) before a wa
 // caller can pass leads outside the operands or gives a row to two groups.
 // Offsets this changes are reported in the device error word. tile0[g] (when
 // given) is the number of `bn`-row tiles of the groups before g, atom0[g] (when
-// given) the number of 128-row tiles before it. All threads of the block call
+// given) the number of 128-row tiles before it. Without offsets there is one
+// group, all rows. All threads of the block call
 // it; the results are visible to all of them when it returns.
 __device__ __forceinline__ void plan_groups(const int *offsets, int groups, int rows, int bn, int *start, int *tile0,
                                             int *atom0, unsigned *dwords) {
-  for (int j = threadIdx.x; j <= groups; j += blockDim.x) start[j] = offsets[j];
+  for (int j = threadIdx.x; j <= groups; j += blockDim.x) start[j] = offsets ? offsets[j] : (j ? rows : 0);
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
@@ -101,6 +102,10 @@ __device__ __forceinline__ int group_of(const int *tile0, int groups, int q) {
     else hi = mid;
   }
   return lo;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(wgtc::smem_addr(bar)) : "memory");
 }
 
 // ---- epilogue ----------------------------------------------------------------
