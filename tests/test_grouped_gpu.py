@@ -157,6 +157,29 @@ def test_rows_longer_contraction_and_many_tiles(wg, device):
     run_rows(wg, device, N, [700, 1, 900], 1000, 2048, "float16", "float32")
 
 
+# Enough tiles, and rows a group, for the CTA-pair form (256 x 256 tiles).
+WIDE = [150, 0, 1, 290, 256, 257, 31, 140, 513, 160, 64, 130, 129, 200, 300]
+
+
+@pytest.mark.parametrize("trans", [T, N])
+@pytest.mark.parametrize("n,k", [(2048, 72), (2056, 136), (1800, 200)])
+@pytest.mark.parametrize("ctype", ["bfloat16", "float32"])
+def test_rows_pairs(wg, device, trans, n, k, ctype):
+    run_rows(wg, device, trans, WIDE, n, k, ctype=ctype, first=1, after=5)
+    run_rows(wg, device, trans, WIDE, n, k, ctype=ctype, alpha=0.5, beta=-1.0, pad=(8, 16, 24, 3))
+
+
+def test_rows_pairs_long(wg, device):
+    run_rows(wg, device, T, [700, 300], 9600, 2048, ctype="float32")
+    run_rows(wg, device, N, [700, 300], 9600, 2056, "float16")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_odd_many_tiles_and_long(wg, device, dtype):
+    run_rows(wg, device, T, [700, 300], 1001, 2049, dtype, "float32")
+    run_rows(wg, device, N, [700, 1, 300], 1001, 1999, dtype)
+
+
 def run_inner(wg, device, sizes, m, n, dtype="bfloat16", ctype="float32", alpha=1.0, beta=0.0, pad=(0, 0, 0, 0), first=0,
               after=0, seed=2, poison=None):
     rng = np.random.default_rng(seed)
@@ -212,6 +235,19 @@ def test_inner_scalars_and_types(wg, device, dtype, ctype, alpha, beta):
 @pytest.mark.parametrize("pad", [(8, 16, 5, 3), (3, 1, 0, 0), (0, 0, 7, 9)])
 def test_inner_strides(wg, device, pad):
     run_inner(wg, device, [33, 0, 70], 136, 200, pad=pad)
+
+
+@pytest.mark.parametrize("m,n", [(520, 776), (264, 1288), (512, 1024)])
+@pytest.mark.parametrize("ctype", ["bfloat16", "float32"])
+def test_inner_pairs(wg, device, m, n, ctype):
+    sizes = [150, 0, 1, 17, 63, 64, 65, 512, 513, 530, 128, 1100, 16, 31, 700, 5]
+    run_inner(wg, device, sizes, m, n, ctype=ctype, first=2, after=3, poison=np.nan)
+    run_inner(wg, device, sizes, m, n, ctype=ctype, alpha=0.5, beta=1.0, pad=(8, 16, 3, 5))
+
+
+def test_inner_long(wg, device):
+    run_inner(wg, device, [5000, 3], 264, 392)
+    run_inner(wg, device, [5000, 3], 263, 391, "float16")
 
 
 @pytest.mark.parametrize("poison", [np.inf, np.nan])

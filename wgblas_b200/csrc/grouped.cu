@@ -6,10 +6,17 @@
 //   rows form:   C[r] = alpha * A[r] op(B_g) + beta * C[r]     r in group g's rows
 //   inner form:  C_g  = alpha * A[rows of g]^T B[rows of g] + beta * C_g
 //
-// One persistent kernel: each CTA walks 128-lane x BN-column tiles (frame and
-// numbering: grouped_common.cuh). Warp 0 streams 64-deep k-blocks of both
-// operands into a ring (TMA, 128-byte swizzle), warp 1 issues tcgen05.mma into
-// one of two TMEM accumulators, warps 2-5 store the other one.
+// One persistent kernel over 128-lane (256 for a CTA pair) x BN-column tiles
+// (frame and numbering: grouped_common.cuh). Warp 0 streams 64-deep k-blocks of
+// both operands into a ring (TMA, 128-byte swizzle), warp 1 issues tcgen05.mma
+// into one of two TMEM accumulators, warps 2-9 add up and store the other one.
+// Forms:
+//   pairs, BN 256   compute-bound calls. A 128 x 256 tile on one CTA needs 96
+//                   bytes of operands a clock from L2, more than an SM gets; a
+//                   pair's 256 x 256 tile needs 64.
+//   one CTA         calls with few rows a group, bound by the weights' bytes.
+// Operands that a TMA map cannot describe (odd row lengths, unaligned bases) are
+// first copied to aligned rows in a stream-ordered temporary.
 #include <algorithm>
 #include <cstring>
 
@@ -22,8 +29,13 @@ using wgg::mbar_arrive;
 using wgg::WAIT_BUDGET;
 
 constexpr int BK = 64;          // k-block: 64 16-bit elements, one 128-byte swizzle span
-constexpr int EPI_WARPS = 4;
-constexpr int LOAD_WARPS = 4;   // of the form that loads with plain loads
+constexpr int EPI_WARPS = wgg::EPI_WARPS;
+// fp32 results: the tensor core truncates when it adds to the accumulator, about
+// 1e-9 of the result a contraction row (measured on normal data: 1.0e-6 at 1024
+// rows, 9.1e-6 at 8192). So accumulators are drained every SEG k-blocks and the
+// drained sums added in registers, rounded to nearest. 16-bit results round at
+// 2^-9 or 2^-11 and need no more than one accumulator.
+constexpr int SEG = 8;
 constexpr int CHUNK = 8192;     // bytes of 64 lines of one k-block
 constexpr size_t SMEM_LIMIT = 227 * 1024;
 
@@ -34,21 +46,23 @@ constexpr size_t SMEM_LIMIT = 227 * 1024;
 //   INNER   both MN-major (rows of A and of B are the contraction)
 enum { ROWS_T = 0, ROWS_N = 1, INNER = 2 };
 
-template <int BN_>
+template <int CG_, int BN_>
 struct Shape {
-  static constexpr int BN = BN_;
+  static constexpr int CG = CG_, BN = BN_;
+  static constexpr int TL = CG * BL;            // lanes of a tile
+  static constexpr int CPT = BN / 2;            // accumulator columns of an epilogue thread
   static constexpr int L_BYTES = BL * 128;
-  static constexpr int N_BYTES = BN * 128;
+  static constexpr int N_BYTES = BN / CG * 128;  // each CTA of a pair holds half of the columns' lines
   static constexpr int STAGE = L_BYTES + N_BYTES;
-  static constexpr int ACC_COLS = BN < 32 ? 32 : BN;
   static constexpr int MAX_STAGES = 10;
   // Ring depth: what shared memory holds beside the groups' tables.
   static constexpr int STAGES = (int)((SMEM_LIMIT - 12 * 1024) / STAGE) < MAX_STAGES
                                     ? (int)((SMEM_LIMIT - 12 * 1024) / STAGE)
                                     : MAX_STAGES;
-  static constexpr size_t smem(int groups) {
-    return 1024 + (size_t)STAGES * STAGE + 256 + 2 * ((size_t)groups + 1) * sizeof(int);
-  }
+  static constexpr int BARS = 4 * STAGES + 4;
+  static constexpr size_t tables = (size_t)STAGES * STAGE + (BARS * 8 + 8 + 15) / 16 * 16;
+  static constexpr size_t smem(int groups) { return 1024 + tables + 2 * ((size_t)groups + 1) * sizeof(int); }
+  static constexpr int NMMA_STEP = CG * 16;
 };
 
 struct Args {
@@ -65,7 +79,7 @@ struct Args {
   int ctype;
   uint32_t ab_format;  // idesc a/b format: 0 fp16, 1 bf16
   int l_group;         // 1: the L side's map has a group dimension (0: all groups share one matrix)
-  // the operands for the plain-load form
+  // the operands
   const uint16_t *L, *N;
   int64_t ldl, ldn, strideL;
   unsigned *dwords;
@@ -87,17 +101,26 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
          (1ull << 46) | (2ull << 61);
 }
 
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
-// One output tile: lanes [l0, l0 + 128) and columns [n0, n0 + nv) of group g,
+// One output tile: lanes [l0, l0 + TL) and columns [n0, n0 + nv) of group g,
 // whose contraction (inner form) or rows (rows form) begin at row r0.
 struct Tile {
   int g, l0, n0, nv;
@@ -114,7 +137,7 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
     x.g = (int)(t / per);
     const int local = (int)(t - (int64_t)x.g * per);
     const int tn = local % a.tiles_n;
-    x.l0 = (local / a.tiles_n) * BL;
+    x.l0 = (local / a.tiles_n) * S::TL;
     x.n0 = tn * S::BN;
     x.nv = min(S::BN, a.nn - x.n0);
     x.r0 = start[x.g];
@@ -126,291 +149,335 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
     const int local = (int)(t - (int64_t)tile0[x.g] * a.tiles_l);
     // The group's row tiles side by side, so that one tile of weights is read
     // by CTAs running at the same time.
-    x.l0 = (local / ntok) * BL;
-    const int first = (local % ntok) * S::BN;
+    x.l0 = (local / ntok) * S::TL;
+    // The group's rows are divided evenly among its tiles: a last tile of a few
+    // rows would load as many weights as a full one.
+    const int rows = start[x.g + 1] - start[x.g];
+    const int each = ((rows + ntok - 1) / ntok + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
+    const int first = (local % ntok) * each;
     x.r0 = start[x.g] + first;
     x.n0 = first;
-    x.nv = min(S::BN, start[x.g + 1] - x.r0);
+    x.nv = min(each, rows - first);
     x.klen = a.k;
   }
   x.kt = a.alpha == 0.0f ? 0 : (x.klen + BK - 1) / BK;
   return x;
 }
 
-// Eight 16-bit elements at p, of which the first `valid` exist (the others are
-// zero), by the widest loads p's alignment allows.
-__device__ __forceinline__ uint4 load8(const uint16_t *p, int valid) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (valid <= 0) return v;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-  if (valid >= 8 && (at & 15) == 0) return __ldg(reinterpret_cast<const uint4 *>(p));
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (valid >= 8 && (at & 3) == 0) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (i < valid) w[i >> 1] |= (uint32_t)__ldg(p + i) << (16 * (i & 1));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// The lines past a group's last row hold the next group's (whatever they are,
+// infinities among them): zeroes those the last MMA of a k-block with `left`
+// lines would read, in `chunks` 64-element chunks. A whole warp calls it.
+__device__ __forceinline__ void zero_tail(uint8_t *st, int left, int chunks, int lane) {
+  const int end = (left + 15) & ~15;
+  for (int q = 0; q < chunks; q++)
+    for (int r = left + (lane >> 3); r < end; r += 4)
+      *reinterpret_cast<uint4 *>(st + q * CHUNK + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+  wgtc::fence_proxy_async_smem();
+  __syncwarp();
 }
 
-template <int MODE, class S, bool TMA>
-__global__ void __launch_bounds__(TMA ? 192 : 320, 1)
+// SUMS: accumulators are drained every SEG k-blocks (fp32 results).
+// Warps: 0 and 10 load (the L and the N side), 1 issues the MMAs, 2-9 store, 11
+// (inner form) zeroes what is past a group's last row.
+template <int MODE, class S, bool SUMS>
+__global__ void __launch_bounds__(MODE == INNER ? 384 : 352, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n, const Args a) {
   constexpr bool L_MN = MODE != ROWS_T, N_MN = MODE == INNER;
-  constexpr int STAGES = S::STAGES;
-  constexpr int NBOX = S::BN < 64 ? S::BN : 64;  // rows of one N-side box
+  constexpr int STAGES = S::STAGES, CG = S::CG;
+  constexpr int NBOX = S::BN < 64 ? S::BN : 64;  // lines of one N-side box
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = wgtc::smem_addr(smem_raw);
   uint8_t *smem = smem_raw + ((1024 - (base & 1023)) & 1023);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + (size_t)STAGES * S::STAGE);
   uint64_t *empty = full + STAGES;
-  uint64_t *acc_full = empty + STAGES;  // [2]
-  uint64_t *acc_empty = acc_full + 2;   // [2]
+  uint64_t *tail = empty + STAGES;       // inner form: this CTA's ragged last block has landed
+  uint64_t *tail_peer = tail + STAGES;   // ... and the other CTA of a pair has zeroed what is past its end
+  uint64_t *acc_full = tail_peer + STAGES;  // [2]
+  uint64_t *acc_empty = acc_full + 2;       // [2]
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  int *start = reinterpret_cast<int *>(smem + (size_t)STAGES * S::STAGE + 256);
+  int *start = reinterpret_cast<int *>(smem + S::tables);
   int *tile0 = start + a.groups + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = wgg::pair_rank<CG>();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
-      wgtc::mbar_init(&full[s], TMA ? 1 : 32 * LOAD_WARPS);
+      wgtc::mbar_init(&full[s], 2);
       wgtc::mbar_init(&empty[s], 1);
+      wgtc::mbar_init(&tail[s], 2);
+      wgtc::mbar_init(&tail_peer[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       wgtc::mbar_init(&acc_full[b], 1);
-      wgtc::mbar_init(&acc_empty[b], 32 * EPI_WARPS);
+      wgtc::mbar_init(&acc_empty[b], CG * EPI_WARPS);
     }
     *abort_flag = 0;
     wgtc::fence_barrier_init();
   }
-  if (TMA && warp == 0 && lane == 0) {
-    wgtc::prefetch_tensormap(&map_l);
-    wgtc::prefetch_tensormap(&map_n);
-  }
-  if (warp == 1) {
-    wgtc::tmem_alloc(tmem_slot, 2 * S::ACC_COLS);
-    wgtc::tmem_relinquish();
-  }
+  if (warp == 0 && lane == 0) wgtc::prefetch_tensormap(&map_l);
+  if (warp == 10 && lane == 0) wgtc::prefetch_tensormap(&map_n);
+  if (warp == 1) wgg::pair_tmem_alloc<CG>(tmem_slot, 2 * S::BN);
   wg_pdl_wait();
   wg_pdl_trigger();
   wgg::plan_groups(a.offsets, a.groups, a.rows, S::BN, start, MODE == INNER ? nullptr : tile0, nullptr, a.dwords);
   wgtc::tc_fence_before();
-  __syncthreads();
+  wgg::pair_sync<CG>();
   wgtc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int64_t tiles = MODE == INNER ? (int64_t)a.groups * a.tiles_l * a.tiles_n
                                       : (int64_t)tile0[a.groups] * a.tiles_l;
+  const int64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
 
-  if (TMA && warp == 0 && lane == 0) {
-    // ---- TMA producer ----
-    int64_t it = 0;
-    bool ok = true;
-    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile x = tile_at<MODE, S>(a, t, start, tile0);
-      const int boxes = (x.nv + NBOX - 1) / NBOX;
-      const uint32_t bytes = (uint32_t)(S::L_BYTES + boxes * NBOX * 128);
-      for (int kb = 0; kb < x.kt; kb++, it++) {
-        const int s = (int)(it % STAGES);
-        const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
-        if (!wgtc::mbar_wait_bounded(&empty[s], ph ^ 1u, WAIT_BUDGET) || *abort_flag) {
-          atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_TMA_WAIT);
-          *abort_flag = 1;
-          ok = false;
-          break;
-        }
-        uint8_t *st = smem + (size_t)s * S::STAGE;
-        wgtc::mbar_arrive_expect_tx(&full[s], bytes);
-        const int k0 = kb * BK;
-        if (MODE == ROWS_T) {
-          wgtc::tma_load_3d(st, &map_l, &full[s], k0, x.l0, x.g * a.l_group);
-        } else if (MODE == ROWS_N) {
-          wgtc::tma_load_3d(st, &map_l, &full[s], x.l0, k0, x.g * a.l_group);
-          wgtc::tma_load_3d(st + CHUNK, &map_l, &full[s], x.l0 + 64, k0, x.g * a.l_group);
-        } else {
-          wgtc::tma_load_2d(st, &map_l, &full[s], x.l0, x.r0 + k0);
-          wgtc::tma_load_2d(st + CHUNK, &map_l, &full[s], x.l0 + 64, x.r0 + k0);
-        }
-        uint8_t *sn = st + S::L_BYTES;
-        for (int b = 0; b < boxes; b++) {
-          if (N_MN) wgtc::tma_load_2d(sn + b * CHUNK, &map_n, &full[s], x.n0 + b * 64, x.r0 + k0);
-          else wgtc::tma_load_2d(sn + b * NBOX * 128, &map_n, &full[s], k0, x.r0 + b * NBOX);
-        }
-      }
-    }
-    // Let every copy this thread issued land before the CTA can exit.
-    for (int64_t q = it - STAGES > 0 ? it - STAGES : 0; q < it; q++)
-      wgtc::mbar_wait_bounded(&full[q % STAGES], (uint32_t)(q / STAGES) & 1u, WAIT_BUDGET);
-  } else if (!TMA && warp >= 6) {
-    // ---- plain-load producer: four warps fill the same swizzled layout, zeros
-    // outside the operands; any alignment ----
-    const int tid = threadIdx.x - 192;
-    int64_t it = 0;
-    bool ok = true;
-    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile x = tile_at<MODE, S>(a, t, start, tile0);
-      const int nmma = (x.nv + 15) & ~15;
-      const uint16_t *Lg = a.L + (int64_t)x.g * a.strideL;
-      for (int kb = 0; kb < x.kt; kb++, it++) {
-        const int s = (int)(it % STAGES);
-        const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
-        ok = wgtc::mbar_wait_bounded(&empty[s], ph ^ 1u, WAIT_BUDGET) && *abort_flag == 0;
-        if (!ok) {
-          atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_TMA_WAIT);
-          *abort_flag = 1;
-          break;
-        }
-        uint8_t *st = smem + (size_t)s * S::STAGE;
-        const int k0 = kb * BK, kleft = x.klen - k0;
-        const int nlines = N_MN ? 64 * ((nmma + 63) / 64) : nmma;
-        const int units = (BL + nlines) * 8;
-#pragma unroll 4
-        for (int u = tid; u < units; u += 32 * LOAD_WARPS) {
-          const int line = u >> 3, c = u & 7;
-          const uint16_t *p;
-          int valid;
-          uint32_t dst;
-          if (line < BL) {
-            if (MODE == ROWS_T) {  // weight row l0 + line, columns k0 ..
-              valid = x.l0 + line < a.nl ? kleft - c * 8 : 0;
-              p = Lg + (int64_t)(x.l0 + line) * a.ldl + k0 + c * 8;
-              dst = line * 128 + ((c ^ (line & 7)) << 4);
-            } else {  // k line kk, columns l0 + 64 * chunk ..
-              const int kk = line & 63, q = line >> 6, col = x.l0 + q * 64 + c * 8;
-              valid = kk < kleft ? a.nl - col : 0;
-              p = (MODE == INNER ? a.L + (int64_t)(x.r0 + k0 + kk) * a.ldl : Lg + (int64_t)(k0 + kk) * a.ldl) + col;
-              dst = q * CHUNK + kk * 128 + ((c ^ (kk & 7)) << 4);
+  // A wait that gives up records it and tells the other roles to stop at their
+  // next failed wait (each is bounded on its own).
+  auto gave_up = [&](unsigned bit) {
+    atomicOr(a.dwords + WG_DW_ERROR, bit);
+    *abort_flag = 1;
+  };
+
+  if (warp == 0 || warp == 10) {
+    if (lane == 0) {
+      // ---- producers: each CTA of a pair loads its own lanes and its half of the columns ----
+      wgg::Ring<STAGES> ring;
+      bool ok = true;
+      const bool l_side = warp == 0;
+      const uint32_t lead = wgg::leader_addr<CG>(full);
+      for (int64_t t = t_first; t < tiles && ok; t += t_step) {
+        const Tile x = tile_at<MODE, S>(a, t, start, tile0);
+        const int half = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
+        // The first box's outer coordinate, and how many boxes.
+        const int c0 = l_side ? x.l0 + (int)rank * BL : (N_MN ? x.n0 : x.r0) + (int)rank * half;
+        const int boxes = l_side ? 2 : (half + NBOX - 1) / NBOX;
+        const uint32_t bytes = (uint32_t)(l_side ? S::L_BYTES : boxes * NBOX * 128);
+        const int lg = x.g * a.l_group;
+        for (int kb = 0; kb < x.kt; kb++, ring.next()) {
+          const int s = ring.s;
+          ok = wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET);
+          if (!ok) {
+            gave_up(WG_DERR_TMA_WAIT);
+            break;
+          }
+          uint8_t *dst = smem + (size_t)s * S::STAGE + (l_side ? 0 : S::L_BYTES);
+          const int k0 = (MODE == INNER ? x.r0 : 0) + kb * BK;
+          if (MODE == INNER && x.klen - kb * BK < BK && (x.klen & 15)) {
+            // A ragged end goes by way of warp 11.
+            wgtc::mbar_arrive_expect_tx(&tail[s], bytes);
+            for (int b = 0; b < boxes; b++)
+              wgtc::tma_load_2d(dst + b * CHUNK, l_side ? &map_l : &map_n, &tail[s], c0 + b * 64, k0);
+            continue;
+          }
+          if (rank == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
+          const uint32_t at = lead + 8u * (uint32_t)s;
+          if (l_side) {
+            if (MODE == ROWS_T) {
+              wgg::load_3d<CG>(dst, &map_l, &full[s], at, k0, c0, lg);
+            } else if (MODE == ROWS_N) {
+              wgg::load_3d<CG>(dst, &map_l, &full[s], at, c0, k0, lg);
+              wgg::load_3d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0, lg);
+            } else {
+              wgg::load_2d<CG>(dst, &map_l, &full[s], at, c0, k0);
+              wgg::load_2d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0);
             }
           } else {
-            const int l = line - BL;
-            if (N_MN) {
-              const int kk = l & 63, q = l >> 6, col = x.n0 + q * 64 + c * 8;
-              valid = kk < kleft ? a.nn - col : 0;
-              p = a.N + (int64_t)(x.r0 + k0 + kk) * a.ldn + col;
-              dst = S::L_BYTES + q * CHUNK + kk * 128 + ((c ^ (kk & 7)) << 4);
-            } else {
-              valid = l < x.nv ? kleft - c * 8 : 0;
-              p = a.N + (int64_t)(x.r0 + l) * a.ldn + k0 + c * 8;
-              dst = S::L_BYTES + l * 128 + ((c ^ (l & 7)) << 4);
+            for (int b = 0; b < boxes; b++) {
+              if (N_MN) wgg::load_2d<CG>(dst + b * CHUNK, &map_n, &full[s], at, c0 + b * 64, k0);
+              else wgg::load_2d<CG>(dst + b * NBOX * 128, &map_n, &full[s], at, k0, c0 + b * NBOX);
             }
           }
-          *reinterpret_cast<uint4 *>(st + dst) = load8(p, valid);
         }
-        wgtc::fence_proxy_async_smem();
-        mbar_arrive(&full[s]);
       }
+      // Let every copy (of both CTAs) land before the CTA can exit: the MMAs that
+      // read a stage complete after its copies, and free it.
+      for (int i = 0; i < STAGES && ok; i++, ring.next())
+        if (!wgtc::mbar_wait_bounded(&empty[ring.s], ring.round ^ 1u, WAIT_BUDGET)) break;
     }
-  } else if (warp == 1) {
-    // ---- MMA issuer (the whole warp, for the zero rows of a ragged end; lane 0 issues) ----
-    int64_t it = 0;
-    int used = 0;
-    bool ok = true;
-    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+  } else if (MODE == INNER && warp == 11) {
+    // ---- ragged ends: zeroes the lines past a group's last row, then hands the stage on ----
+    int s = 0;
+    uint32_t phase = 0;  // parity of tail[s], tail_peer[s] at bit s
+    for (int64_t t = t_first; t < tiles; t += t_step) {
       const Tile x = tile_at<MODE, S>(a, t, start, tile0);
       if (x.kt == 0) continue;
-      const int nmma = (x.nv + 15) & ~15;
-      const uint32_t idesc = idesc_f16(a.ab_format, BL, nmma, L_MN, N_MN);
-      const int b = used & 1;
-      ok = wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET) && *abort_flag == 0;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        if (lane == 0) atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_MMA_WAIT);
-        *abort_flag = 1;
-        break;
-      }
-      wgtc::tc_fence_after();
-      const uint32_t d_tmem = tmem + (uint32_t)(b * S::ACC_COLS);
-      for (int kb = 0; kb < x.kt; kb++, it++) {
-        const int s = (int)(it % STAGES);
-        ok = wgtc::mbar_wait_bounded(&full[s], (uint32_t)(it / STAGES) & 1u, WAIT_BUDGET) && *abort_flag == 0;
-        ok = __all_sync(0xffffffffu, ok);
+      s = (s + x.kt - 1) % STAGES;  // the tile's last block
+      const int left = x.klen - (x.kt - 1) * BK;
+      if (left & 15) {
+        const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
+        bool ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&tail[s], phase >> s & 1u, WAIT_BUDGET));
+        if (ok) {
+          zero_tail(smem + (size_t)s * S::STAGE, left, 2 + (nmma / CG + 63) / 64, lane);
+          if (CG == 2 && rank == 1) {
+            if (lane == 0) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(&tail_peer[s]), 0));
+          } else {
+            if (CG == 2)
+              ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(&tail_peer[s], phase >> s & 1u, WAIT_BUDGET));
+            if (ok && lane == 0)
+              asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(wgtc::smem_addr(&full[s])) : "memory");
+          }
+        }
         if (!ok) {
-          if (lane == 0) atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_TMA_WAIT);
-          *abort_flag = 1;
+          if (lane == 0) gave_up(WG_DERR_TMA_WAIT);
           break;
         }
-        uint8_t *st = smem + (size_t)s * S::STAGE;
-        const int left = min(BK, x.klen - kb * BK);
-        const int steps = (left + 15) >> 4;
-        if (TMA && MODE == INNER && (left & 15)) {
-          // The lines past the group's last row hold the next group's (whatever
-          // they are, infinities among them): zero those the last MMA would read.
-          const int lines = steps * 16 - left, chunks = 2 + (nmma + 63) / 64;
-          for (int u = lane; u < chunks * lines * 8; u += 32) {
-            const int c = u & 7, r = (u >> 3) % lines, q = (u >> 3) / lines;
-            *reinterpret_cast<uint4 *>(st + q * CHUNK + (left + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-          }
-          wgtc::fence_proxy_async_smem();
-          __syncwarp();
-        }
-        wgtc::tc_fence_after();
-        if (lane == 0) {
-          const uint32_t sl = wgtc::smem_addr(st), sn = sl + S::L_BYTES;
-          for (int kk = 0; kk < steps; kk++) {
-            const uint64_t dl = L_MN ? smem_desc_mn(sl + kk * 2048) : wgtc::smem_desc_kmajor(sl + kk * 32, 128);
-            const uint64_t dn = N_MN ? smem_desc_mn(sn + kk * 2048) : wgtc::smem_desc_kmajor(sn + kk * 32, 128);
-            mma_f16(d_tmem, dl, dn, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-          }
-          wgtc::mma_commit(&empty[s]);
-        }
-        __syncwarp();
+        phase ^= 1u << s;
       }
-      if (!ok) break;
-      if (lane == 0) wgtc::mma_commit(&acc_full[b]);
-      used++;
+      if (++s == STAGES) s = 0;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      // ---- MMA issuer ----
+      wgg::Ring<STAGES> ring;
+      int used = 0;
+      constexpr int segment = SUMS ? SEG : 1 << 30;
+      constexpr uint64_t step_l = (L_MN ? 2048 : 32) >> 4, step_n = (N_MN ? 2048 : 32) >> 4;
+      const uint32_t smem0 = wgtc::smem_addr(smem);
+      const uint64_t desc_l0 = L_MN ? smem_desc_mn(smem0) : wgtc::smem_desc_kmajor(smem0, 128);
+      const uint64_t desc_n0 = N_MN ? smem_desc_mn(smem0 + S::L_BYTES) : wgtc::smem_desc_kmajor(smem0 + S::L_BYTES, 128);
+      bool ok = true;
+      for (int64_t t = t_first; t < tiles && ok; t += t_step) {
+        const Tile x = tile_at<MODE, S>(a, t, start, tile0);
+        const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
+        const uint32_t idesc = idesc_f16(a.ab_format, S::TL, nmma, L_MN, N_MN);
+        for (int kb0 = 0; kb0 < x.kt && ok; kb0 += segment, used++) {
+          const int b = used & 1, kb1 = min(x.kt, kb0 + segment);
+          const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
+          ok = wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET);
+          wgtc::tc_fence_after();
+          uint32_t more = 0;
+          for (int kb = kb0; kb < kb1 && ok; kb++, ring.next()) {
+            ok = wgtc::mbar_wait_bounded(&full[ring.s], ring.round, WAIT_BUDGET);
+            if (!ok) break;
+            wgtc::tc_fence_after();
+            const uint64_t at = (uint64_t)((uint32_t)ring.s * (S::STAGE >> 4));
+            const uint64_t dl = desc_l0 + at, dn = desc_n0 + at;
+            const int steps = (x.klen - kb * BK + 15) >> 4;
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              if (kk < steps) {
+                mma_f16<CG>(d_tmem, dl + kk * step_l, dn + kk * step_n, idesc, more);
+                more = 1;
+              }
+            wgg::commit<CG>(&empty[ring.s]);
+          }
+          if (ok) wgg::commit<CG>(&acc_full[b]);
+        }
+      }
+      if (!ok) gave_up(WG_DERR_MMA_WAIT);
     }
   } else if (warp >= 2 && warp < 2 + EPI_WARPS) {
     // ---- epilogue ----
-    const int q = warp & 3;
+    const int q = warp & 3, h = (warp - 2) >> 2;
     int used = 0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    bool ok = true;
+    auto wait_acc = [&](int b) {
+      bool got = wgtc::mbar_wait_bounded(&acc_full[b], (uint32_t)(used >> 1) & 1u, WAIT_BUDGET) && *abort_flag == 0;
+      got = __all_sync(0xffffffffu, got);
+      if (!got && lane == 0) gave_up(WG_DERR_MMA_WAIT);
+      wgtc::tc_fence_after();
+      return got;
+    };
+    auto free_acc = [&](int b) {
+      wgtc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) wgg::leader_arrive<CG>(&acc_empty[b]);
+      used++;
+    };
+    for (int64_t t = t_first; t < tiles && ok; t += t_step) {
       const Tile x = tile_at<MODE, S>(a, t, start, tile0);
-      const int b = used & 1;
-      bool ready = true;
-      if (x.kt) {
-        ready = wgtc::mbar_wait_bounded(&acc_full[b], (uint32_t)(used >> 1) & 1u, WAIT_BUDGET) && *abort_flag == 0;
-        ready = __all_sync(0xffffffffu, ready);
-        if (!ready) {
-          if (lane == 0) atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_MMA_WAIT);
-          *abort_flag = 1;
-          break;
-        }
-        wgtc::tc_fence_after();
-      }
-      const int l = x.l0 + q * 32 + lane;
-      const int64_t row = MODE == INNER ? x.n0 : x.r0;
+      const int valid = x.nv - h * S::CPT;  // columns this warp has (may be none)
+      const int l = x.l0 + (int)rank * BL + q * 32 + lane;
+      const int64_t row = (MODE == INNER ? x.n0 : x.r0) + h * S::CPT;
       const int64_t at = (MODE == INNER ? (int64_t)x.g * a.strideC : 0) + row * a.ldc + l;
-      const uint32_t trow = tmem + (uint32_t)(b * S::ACC_COLS) + ((uint32_t)(q * 32) << 16);
-      for (int c = 0; c < x.nv; c += 32) {
-        uint32_t r[32];
-        if (x.kt) {
-          wgtc::tmem_ld_32x32b_x32(trow + (uint32_t)c, r);
-          wgtc::tmem_ld_wait();
-        } else {
+      const uint32_t col = tmem + (uint32_t)(h * S::CPT) + ((uint32_t)(q * 32) << 16);
+      if constexpr (SUMS) {
+        float sum[S::CPT];
 #pragma unroll
-          for (int j = 0; j < 32; j++) r[j] = 0;
+        for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
+        for (int kb0 = 0; kb0 < x.kt; kb0 += SEG) {
+          const int b = used & 1;
+          if (!(ok = wait_acc(b))) break;
+          wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == 0, sum);
+          free_acc(b);
         }
-        if (l < a.nl) wgg::store_cols<32>(a.C, a.ctype, at + (int64_t)c * a.ldc, a.ldc, x.nv - c, a.alpha, a.beta, r);
-      }
-      if (x.kt) {
-        wgtc::tc_fence_before();
-        mbar_arrive(&acc_empty[b]);
-        used++;
+        if (ok && l < a.nl) wgg::store_sums<S::CPT>(static_cast<float *>(a.C) + at, a.ldc, valid, a.alpha, a.beta, sum);
+      } else {
+        const int b = used & 1;
+        if (x.kt && !(ok = wait_acc(b))) break;
+        wgg::store_acc<S::CPT>(col + (uint32_t)(b * S::BN), x.kt != 0, a.C, a.ctype, at, a.ldc, valid, l < a.nl, a.alpha,
+                               a.beta);
+        if (x.kt) free_acc(b);
       }
     }
   }
 
   wgtc::tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  wgg::pair_sync<CG>();
   if (warp == 1) {
-    __syncwarp();
     wgtc::tc_fence_after();
-    wgtc::tmem_dealloc(tmem, 2 * S::ACC_COLS);
+    wgg::pair_tmem_dealloc<CG>(tmem, 2 * S::BN);
   }
 }
+
+// ---- rows of any alignment to rows of whole 16-byte units --------------------
+
+struct Realign {
+  const uint16_t *src;
+  uint16_t *dst;
+  int64_t ld, stride, ld_out;
+  int64_t lines;      // rows of all matrices together
+  int rows, cols;     // of one matrix
+  const int *offsets;  // matrices of groups without rows are not copied (NULL: all are)
+};
+
+// Elements e .. e + 7 of a line (`cols` long) at p; aligned 16-byte loads, moved
+// into place by words and half words. Memory outside [lo, hi) is not read.
+__device__ __forceinline__ uint4 load8(const uint16_t *p, int valid, const uint16_t *lo, const uint16_t *hi) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const uint16_t *base = reinterpret_cast<const uint16_t *>(at & ~(uintptr_t)15);
+  const int s = (int)(at & 15) >> 1;  // elements before p in its 16-byte unit
+  if (s == 0 && valid >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+  if (base >= lo && base + 16 <= hi) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(base)), b = __ldg(reinterpret_cast<const uint4 *>(base) + 1);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (s & 2)
+#pragma unroll
+      for (int i = 0; i < 7; i++) w[i] = w[i + 1];
+    if (s & 4)
+#pragma unroll
+      for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+    const int sh = (s & 1) * 16;
+    return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh),
+                      __funnelshift_r(w[2], w[3], sh), __funnelshift_r(w[3], w[4], sh));
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < valid) w[i >> 1] |= (uint32_t)__ldg(p + i) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A warp a line. What follows a line's last element in its last unit is never
+// read (the tensor maps end at `cols`).
+__global__ void __launch_bounds__(256) grouped_realign(const Realign x, const Realign y) {
+  wg_pdl_wait();
+  wg_pdl_trigger();
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const bool second = w >= x.lines;
+  const Realign &a = second ? y : x;
+  const int64_t line = second ? w - x.lines : w;
+  if (line >= a.lines) return;
+  const int64_t g = line / a.rows, r = line - g * a.rows;
+  if (a.offsets && a.offsets[g + 1] <= a.offsets[g]) return;
+  const uint16_t *src = a.src + g * a.stride + r * a.ld;
+  const uint16_t *lo = a.src, *hi = a.src + (a.lines / a.rows - 1) * a.stride + (int64_t)(a.rows - 1) * a.ld + a.cols;
+  uint16_t *dst = a.dst + line * a.ld_out;
+#pragma unroll 4
+  for (int e = (threadIdx.x & 31) * 8; e < a.cols; e += 256)
+    *reinterpret_cast<uint4 *>(dst + e) = load8(src + e, a.cols - e, lo, hi);
+}
+
+constexpr int64_t LIM = (int64_t)1 << 31;
 
 // ---- host side ------------------------------------------------------------
 
@@ -425,74 +492,130 @@ bool encode(CUtensorMap *map, int type, const void *ptr, int rank, const cuuint6
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A TMA map can read a row-major matrix whose base and row length are whole
-// 16-byte units (cuTensorMapEncodeTiled's rule; strides below 2^40 bytes).
-bool mappable(const void *p, int64_t ld) {
-  return ((uintptr_t)p & 15) == 0 && (ld * 2) % 16 == 0 && ld * 2 < ((int64_t)1 << 40);
+// A TMA map can read row-major matrices whose base, row length and distance are
+// whole 16-byte units (cuTensorMapEncodeTiled's rule; strides below 2^40 bytes).
+bool mappable(const void *p, int64_t ld, int64_t stride) {
+  return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && stride % 8 == 0 && ld < ((int64_t)1 << 39) &&
+         stride < ((int64_t)1 << 39);
 }
 
+// The tensor maps of a call (mappable operands).
 template <int MODE, class S>
-wg_status launch(wg_device *d, const char *family, Args &a, int type, int64_t row_tiles_most) {
-  const bool l_rows = MODE != INNER;
-  // Weights shared by all groups (stride 0, or one group) need no group dimension.
-  a.l_group = l_rows && a.groups > 1 && a.strideL != 0;
-  bool tma = mappable(a.L, a.ldl) && mappable(a.N, a.ldn) &&
-             (!a.l_group || ((a.strideL * 2) % 16 == 0 && a.strideL * 2 < ((int64_t)1 << 40)));
-  CUtensorMap ml, mn;
-  memset(&ml, 0, sizeof ml);
-  memset(&mn, 0, sizeof mn);
-  if (tma) {
-    const cuuint64_t ldl = (cuuint64_t)a.ldl * 2, ldn = (cuuint64_t)a.ldn * 2;
-    if (MODE == INNER) {
-      const cuuint64_t dl[2] = {(cuuint64_t)a.nl, (cuuint64_t)a.rows}, dn[2] = {(cuuint64_t)a.nn, (cuuint64_t)a.rows};
-      const cuuint32_t box[2] = {64, 64};
-      tma = encode(&ml, type, a.L, 2, dl, &ldl, box) && encode(&mn, type, a.N, 2, dn, &ldn, box);
-    } else {
-      const int64_t lrows = MODE == ROWS_T ? a.nl : a.k, lcols = MODE == ROWS_T ? a.k : a.nl;
-      const cuuint64_t dl[3] = {(cuuint64_t)lcols, (cuuint64_t)lrows, a.l_group ? (cuuint64_t)a.groups : 1};
-      const cuuint64_t sl[2] = {ldl, a.l_group ? (cuuint64_t)a.strideL * 2 : ldl * (cuuint64_t)lrows};
-      const cuuint32_t bl[3] = {64, MODE == ROWS_T ? (cuuint32_t)BL : 64u, 1};
-      const cuuint64_t dn[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
-      const cuuint32_t bn[2] = {64, (cuuint32_t)std::min(S::BN, 64)};
-      tma = encode(&ml, type, a.L, 3, dl, sl, bl) && encode(&mn, type, a.N, 2, dn, &ldn, bn);
-    }
+bool make_maps(const Args &a, int type, CUtensorMap *ml, CUtensorMap *mn) {
+  const cuuint64_t ldl = (cuuint64_t)a.ldl * 2, ldn = (cuuint64_t)a.ldn * 2;
+  if (MODE == INNER) {
+    const cuuint64_t dl[2] = {(cuuint64_t)a.nl, (cuuint64_t)a.rows}, dn[2] = {(cuuint64_t)a.nn, (cuuint64_t)a.rows};
+    const cuuint32_t box[2] = {64, 64};
+    return encode(ml, type, a.L, 2, dl, &ldl, box) && encode(mn, type, a.N, 2, dn, &ldn, box);
   }
-  const size_t smem = S::smem(a.groups);
-  const int64_t most = row_tiles_most * a.tiles_l;
-  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count));
-  wg_launch_scope scope(d, family);
-  if (tma) {
-    WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, true>, SMEM_LIMIT));
-    WG_CUDA(wg_launch_pdl(grouped_kernel<MODE, S, true>, dim3(grid), dim3(192), smem, d->stream, ml, mn, a));
-  } else {
-    WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, false>, SMEM_LIMIT));
-    WG_CUDA(wg_launch_pdl(grouped_kernel<MODE, S, false>, dim3(grid), dim3(320), smem, d->stream, ml, mn, a));
-  }
+  const int64_t lrows = MODE == ROWS_T ? a.nl : a.k, lcols = MODE == ROWS_T ? a.k : a.nl;
+  const cuuint64_t dl[3] = {(cuuint64_t)lcols, (cuuint64_t)lrows, a.l_group ? (cuuint64_t)a.groups : 1};
+  const cuuint64_t sl[2] = {ldl, a.l_group ? (cuuint64_t)a.strideL * 2 : ldl * (cuuint64_t)lrows};
+  const cuuint32_t bl[3] = {64, MODE == ROWS_T ? (cuuint32_t)BL : 64u, 1};
+  const cuuint64_t dn[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows};
+  const cuuint32_t bn[2] = {64, (cuuint32_t)std::min(S::BN, 64)};
+  return encode(ml, type, a.L, 3, dl, sl, bl) && encode(mn, type, a.N, 2, dn, &ldn, bn);
+}
+
+template <int MODE, class S, bool SUMS>
+wg_status launch_as(wg_device *d, Args &a, const CUtensorMap &ml, const CUtensorMap &mn) {
+  a.tiles_l = (a.nl + S::TL - 1) / S::TL;
+  a.tiles_n = MODE == INNER ? (a.nn + S::BN - 1) / S::BN : 0;
+  const int64_t most = (int64_t)a.tiles_l * (MODE == INNER ? (int64_t)a.groups * a.tiles_n
+                                                           : (int64_t)a.rows / S::BN + a.groups);
+  const unsigned grid = S::CG * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CG));
+  wg_launch_scope scope(d, MODE == INNER ? "gemm_grouped_inner" : "gemm_grouped");
+  WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, SUMS>, SMEM_LIMIT));
+  WG_CUDA((wgg::launch<S::CG>(grouped_kernel<MODE, S, SUMS>, grid, MODE == INNER ? 384 : 352, S::smem(a.groups),
+                              d->stream, ml, mn, a)));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
 }
 
-// Columns of a tile: enough for a group's rows when they are spread evenly, as
-// few as its rows fill otherwise.
+template <int MODE, class S>
+wg_status launch(wg_device *d, Args &a, int type) {
+  CUtensorMap ml, mn;
+  memset(&ml, 0, sizeof ml);
+  memset(&mn, 0, sizeof mn);
+  // (no product, no operands)
+  if (a.alpha != 0.0f && !make_maps<MODE, S>(a, type, &ml, &mn))
+    return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
+  // One accumulator holds at most SEG k-blocks' sums of an fp32 result.
+  const bool sums = a.ctype == WG_TYPE_F32 && (MODE == INNER ? a.rows : a.k) > SEG * BK;
+  return sums ? launch_as<MODE, S, true>(d, a, ml, mn) : launch_as<MODE, S, false>(d, a, ml, mn);
+}
+
 template <int MODE>
-wg_status launch_rows(wg_device *d, Args &a, int type) {
-  const int64_t avg = (a.rows + a.groups - 1) / a.groups;
-  if (avg <= 32) return launch<MODE, Shape<32>>(d, "gemm_grouped", a, type, a.rows / 32 + a.groups);
-  if (avg <= 64) return launch<MODE, Shape<64>>(d, "gemm_grouped", a, type, a.rows / 64 + a.groups);
-  if (avg <= 128) return launch<MODE, Shape<128>>(d, "gemm_grouped", a, type, a.rows / 128 + a.groups);
-  return launch<MODE, Shape<256>>(d, "gemm_grouped", a, type, a.rows / 256 + a.groups);
-}
-
-wg_status launch_inner(wg_device *d, Args &a, int type) {
-  a.tiles_n = (a.nn + 255) / 256;
-  if (a.nn <= 128) {
-    a.tiles_n = (a.nn + 127) / 128;
-    return launch<INNER, Shape<128>>(d, "gemm_grouped_inner", a, type, (int64_t)a.groups * a.tiles_n);
+wg_status run(wg_device *d, Args &a, int type) {
+  // Weights shared by all groups (stride 0, or one group) need no group dimension.
+  a.l_group = MODE != INNER && a.groups > 1 && a.strideL != 0;
+  void *temp = nullptr;
+  if (a.alpha != 0.0f) {
+    Realign l = {}, n = {};
+    size_t bytes = 0;
+    if (!mappable(a.L, a.ldl, a.l_group ? a.strideL : 0)) {
+      l.src = a.L;
+      l.ld = a.ldl;
+      l.stride = a.l_group ? a.strideL : 0;
+      l.rows = MODE == INNER ? a.rows : MODE == ROWS_T ? a.nl : a.k;
+      l.cols = MODE == ROWS_T ? a.k : a.nl;
+      l.lines = (int64_t)l.rows * (a.l_group ? a.groups : 1);
+      l.ld_out = ((int64_t)l.cols + 7) / 8 * 8;
+      l.offsets = a.l_group ? a.offsets : nullptr;
+      bytes = (size_t)(l.lines * l.ld_out) * 2;
+    }
+    if (!mappable(a.N, a.ldn, 0)) {
+      n.src = a.N;
+      n.ld = a.ldn;
+      n.rows = a.rows;
+      n.cols = MODE == INNER ? a.nn : a.k;
+      n.lines = n.rows;
+      n.ld_out = ((int64_t)n.cols + 7) / 8 * 8;
+    }
+    const size_t total = bytes + (size_t)(n.lines * n.ld_out) * 2;
+    if (total) {
+      // From the handle's stream-ordered pool: captured into a graph, each graph has its own.
+      wg_status st = wg_staging_pool(d);
+      if (st != WG_OK) return st;
+      WG_CUDA(cudaMallocFromPoolAsync(&temp, total, d->staging, d->stream));
+      if (l.lines) {
+        l.dst = static_cast<uint16_t *>(temp);
+        a.L = l.dst;
+        a.ldl = l.ld_out;
+        if (a.l_group) a.strideL = l.rows * l.ld_out;
+      }
+      if (n.lines) {
+        n.dst = reinterpret_cast<uint16_t *>(static_cast<char *>(temp) + bytes);
+        a.N = n.dst;
+        a.ldn = n.ld_out;
+      }
+      const int64_t blocks = (l.lines + n.lines + 7) / 8;
+      cudaError_t e = blocks < LIM ? cudaSuccess : cudaErrorInvalidValue;
+      if (e == cudaSuccess) {
+        wg_launch_scope scope(d, "grouped_realign");
+        e = wg_launch_pdl(grouped_realign, dim3((unsigned)blocks), dim3(256), 0, d->stream, l, n);
+      }
+      if (e != cudaSuccess) {
+        cudaFreeAsync(temp, d->stream);
+        return wg_fail(WG_ERR_CUDA, "grouped_realign failed: %s", cudaGetErrorString(e));
+      }
+    }
   }
-  return launch<INNER, Shape<256>>(d, "gemm_grouped_inner", a, type, (int64_t)a.groups * a.tiles_n);
+  const int64_t avg = (a.rows + a.groups - 1) / a.groups;
+  // Tiles the pair form would have (rows form: at least).
+  const int64_t pairs = (int64_t)((a.nl + 255) / 256) *
+                        (MODE == INNER ? (int64_t)a.groups * ((a.nn + 255) / 256) : std::max<int64_t>(a.groups, a.rows / 256));
+  const bool pair = (MODE == INNER ? a.nn > 128 : avg > 128) && 2 * pairs >= d->sm_count;
+  wg_status st;
+  if (pair) st = launch<MODE, Shape<2, 256>>(d, a, type);
+  else if (MODE != INNER && avg <= 32) st = launch<MODE, Shape<1, 32>>(d, a, type);
+  else st = launch<MODE, Shape<1, 128>>(d, a, type);
+  if (temp) {
+    const cudaError_t e = cudaFreeAsync(temp, d->stream);
+    if (st == WG_OK) WG_CUDA(e);
+  }
+  return st;
 }
-
-constexpr int64_t LIM = (int64_t)1 << 31;
 
 wg_status check_common(const wg_device *d, int type, int ctype, int64_t groups, int64_t m, int64_t n, int64_t k) {
   if (!d) return wg_fail(WG_ERR_INVALID_ARGUMENT, "device is NULL");
@@ -507,6 +630,13 @@ wg_status check_common(const wg_device *d, int type, int ctype, int64_t groups, 
   // Row and column numbers are 32-bit in the kernels and their copies, with room for one tile.
   if (m >= LIM - 1024 || n >= LIM - 1024 || k >= LIM - 1024)
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "dimensions must be below 2^31 - 1024");
+  return WG_OK;
+}
+
+// Loads and stores go by elements of the operands' types.
+wg_status check_aligned(const void *A, const void *B, const void *C, int ctype) {
+  if (((uintptr_t)A | (uintptr_t)B) & 1 || ((uintptr_t)C & (ctype == WG_TYPE_F32 ? 3 : 1)))
+    return wg_fail(WG_ERR_INVALID_ARGUMENT, "A, B, and C must be aligned to their elements.");
   return WG_OK;
 }
 
@@ -536,6 +666,7 @@ extern "C" wg_status wg_gemm_grouped_dev(wg_device *d, int type, int ctype, int 
   if (groups == 0 || m == 0 || n == 0) return WG_OK;
   if (!offsets || !C || (k > 0 && alpha != 0.0f && (!A || !B)))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
+  if ((st = check_aligned(A, B, C, ctype)) != WG_OK) return st;
   st = wgg::check_arch(d);
   if (st != WG_OK) return st;
   if (beta == 1.0f && (alpha == 0.0f || k == 0)) return WG_OK;  // C stays as it is
@@ -545,7 +676,6 @@ extern "C" wg_status wg_gemm_grouped_dev(wg_device *d, int type, int ctype, int 
   a.rows = (int)m;
   a.nl = (int)n;
   a.k = (int)k;
-  a.tiles_l = (int)((n + BL - 1) / BL);
   a.offsets = offsets;
   a.alpha = k > 0 ? alpha : 0.0f;
   a.beta = beta;
@@ -559,7 +689,7 @@ extern "C" wg_status wg_gemm_grouped_dev(wg_device *d, int type, int ctype, int 
   a.N = static_cast<const uint16_t *>(A);
   a.ldn = lda;
   a.dwords = d->dwords;
-  return wg_timed(d, gpu_ms, [&] { return transB ? launch_rows<ROWS_T>(d, a, type) : launch_rows<ROWS_N>(d, a, type); });
+  return wg_timed(d, gpu_ms, [&] { return transB ? run<ROWS_T>(d, a, type) : run<ROWS_N>(d, a, type); });
 }
 
 extern "C" wg_status wg_gemm_grouped_inner_dev(wg_device *d, int type, int ctype, int64_t groups, int64_t m, int64_t n,
@@ -578,6 +708,7 @@ extern "C" wg_status wg_gemm_grouped_inner_dev(wg_device *d, int type, int ctype
   if (groups == 0 || m == 0 || n == 0) return WG_OK;
   if (!offsets || !C || (k > 0 && alpha != 0.0f && (!A || !B)))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
+  if ((st = check_aligned(A, B, C, ctype)) != WG_OK) return st;
   st = wgg::check_arch(d);
   if (st != WG_OK) return st;
   if (beta == 1.0f && (alpha == 0.0f || k == 0)) return WG_OK;  // C stays as it is
@@ -587,7 +718,6 @@ extern "C" wg_status wg_gemm_grouped_inner_dev(wg_device *d, int type, int ctype
   a.rows = (int)k;
   a.nl = (int)n;
   a.nn = (int)m;
-  a.tiles_l = (int)((n + BL - 1) / BL);
   a.offsets = offsets;
   a.alpha = k > 0 ? alpha : 0.0f;
   a.beta = beta;
@@ -601,5 +731,5 @@ extern "C" wg_status wg_gemm_grouped_inner_dev(wg_device *d, int type, int ctype
   a.N = static_cast<const uint16_t *>(A);
   a.ldn = lda;
   a.dwords = d->dwords;
-  return wg_timed(d, gpu_ms, [&] { return launch_inner(d, a, type); });
+  return wg_timed(d, gpu_ms, [&] { return run<INNER>(d, a, type); });
 }

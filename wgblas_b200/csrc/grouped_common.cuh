@@ -110,45 +110,41 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
 
 // ---- epilogue ----------------------------------------------------------------
 
-// The element types of operands and results (WG_TYPE_* of the C ABI).
-__device__ __forceinline__ float load_c(const void *c, int64_t i, int type) {
-  if (type == WG_TYPE_F32) return static_cast<const float *>(c)[i];
-  if (type == WG_TYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(c)[i]);
-  return __half2float(static_cast<const __half *>(c)[i]);
-}
-
-// Stores W accumulator columns of one lane: row r0 + j of C (ldc apart), for
-// j < valid. alpha, beta as in BLAS (C is read only when beta != 0), in 32
-// bits, rounded once to C's type. `at` points at the lane's element of the
-// first row.
+// Stores W sums of one lane: row r0 + j of C (ldc apart), for j < valid. alpha,
+// beta as in BLAS (C is read only when beta != 0), in 32 bits, rounded once to
+// C's type. `at` points at the lane's element of the first row.
 template <class T, int W, class Round>
-__device__ __forceinline__ void store_typed(T *at, int64_t ldc, int valid, float alpha, float beta,
-                                            const uint32_t (&acc)[W], Round round) {
+__device__ __forceinline__ void store_typed(T *at, int64_t ldc, int valid, float alpha, float beta, const float *acc,
+                                            Round round) {
+  // (pointers step by ldc: W addresses kept apart would not fit the registers)
   if (beta == 0.0f) {
     if (valid >= W) {
 #pragma unroll
-      for (int j = 0; j < W; j++) at[j * ldc] = round(alpha * __uint_as_float(acc[j]));
+      for (int j = 0; j < W; j++, at += ldc) *at = round(alpha * acc[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < W; j++)
-        if (j < valid) at[j * ldc] = round(alpha * __uint_as_float(acc[j]));
+      for (int j = 0; j < W; j++, at += ldc)
+        if (j < valid) *at = round(alpha * acc[j]);
     }
     return;
   }
-  // The old values of a chunk are loaded before any is written: one memory
-  // round trip for the chunk.
-  T old[W];
+  // The old values of eight rows are loaded before any is written: one memory
+  // round trip for them.
 #pragma unroll
-  for (int j = 0; j < W; j++)
-    if (j < valid) old[j] = at[j * ldc];
+  for (int c = 0; c < W; c += 8) {
+    T old[8], *p = at;
 #pragma unroll
-  for (int j = 0; j < W; j++)
-    if (j < valid) at[j * ldc] = round(fmaf(beta, (float)old[j], alpha * __uint_as_float(acc[j])));
+    for (int j = 0; j < 8; j++, p += ldc)
+      if (c + j < valid) old[j] = *p;
+#pragma unroll
+    for (int j = 0; j < 8; j++, at += ldc)
+      if (c + j < valid) *at = round(fmaf(beta, (float)old[j], alpha * acc[c + j]));
+  }
 }
 
 template <int W>
 __device__ __forceinline__ void store_cols(void *C, int type, int64_t at, int64_t ldc, int valid, float alpha,
-                                           float beta, const uint32_t (&acc)[W]) {
+                                           float beta, const float *acc) {
   if (type == WG_TYPE_BF16)
     store_typed<__nv_bfloat16, W>(static_cast<__nv_bfloat16 *>(C) + at, ldc, valid, alpha, beta, acc,
                                   [](float x) { return __float2bfloat16_rn(x); });
@@ -157,6 +153,133 @@ __device__ __forceinline__ void store_cols(void *C, int type, int64_t at, int64_
                            [](float x) { return __float2half_rn(x); });
   else
     store_typed<float, W>(static_cast<float *>(C) + at, ldc, valid, alpha, beta, acc, [](float x) { return x; });
+}
+
+// Eight epilogue warps: warp w of them reads lane quarter w % 4 and its half
+// w / 4 of the columns, CPT of them.
+constexpr int EPI_WARPS = 8;
+
+// sum[] (+)= CPT accumulator columns from TMEM address `taddr`, of which `valid`
+// are used (16 at a time: the sums leave few registers).
+template <int CPT>
+__device__ __forceinline__ void drain(uint32_t taddr, int valid, bool first, float (&sum)[CPT]) {
+#pragma unroll
+  for (int c = 0; c < CPT; c += 16) {
+    if (c < valid) {
+      uint32_t r[16];
+      wgtc::tmem_ld_32x32b_x16(taddr + (uint32_t)c, r);
+      wgtc::tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; j++) sum[c + j] = first ? __uint_as_float(r[j]) : sum[c + j] + __uint_as_float(r[j]);
+    }
+  }
+}
+
+template <int CPT>
+__device__ __forceinline__ void store_sums(float *at, int64_t ldc, int valid, float alpha, float beta,
+                                           const float (&sum)[CPT]) {
+#pragma unroll
+  for (int c = 0; c < CPT; c += 16, at += 16 * ldc)
+    if (c < valid) store_typed<float, 16>(at, ldc, valid - c, alpha, beta, sum + c, [](float x) { return x; });
+}
+
+// Stores CPT accumulator columns straight from TMEM (`from` false: zeros instead).
+template <int CPT>
+__device__ __forceinline__ void store_acc(uint32_t taddr, bool from, void *C, int type, int64_t at, int64_t ldc,
+                                          int valid, bool in, float alpha, float beta) {
+  constexpr int W = CPT < 32 ? CPT : 32;
+  static_assert(W == 16 || W == 32, "");
+#pragma unroll 1
+  for (int c = 0; c < CPT && c < valid; c += W) {
+    uint32_t r[W];
+    float f[W];
+    if (from) {
+      if constexpr (W == 32) wgtc::tmem_ld_32x32b_x32(taddr + (uint32_t)c, r);
+      else wgtc::tmem_ld_32x32b_x16(taddr + (uint32_t)c, r);
+      wgtc::tmem_ld_wait();
+    }
+#pragma unroll
+    for (int j = 0; j < W; j++) f[j] = from ? __uint_as_float(r[j]) : 0.0f;
+    if (in) store_cols<W>(C, type, at + (int64_t)c * ldc, ldc, valid - c, alpha, beta, f);
+  }
+}
+
+// A place in a ring of N stages, and the parity of the round it is in.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      round ^= 1u;
+    }
+  }
+};
+
+// ---- CTA pairs -------------------------------------------------------------------
+//
+// CG CTAs (1 or 2) share a tile of CG * 128 lanes; CTA 0 of a pair leads: it
+// issues the MMAs, and its barriers count both CTAs' bytes and both epilogues.
+
+template <int CG>
+__device__ __forceinline__ uint32_t pair_rank() {
+  if constexpr (CG == 2) return wgtc::cluster_ctarank();
+  else return 0;
+}
+template <int CG>
+__device__ __forceinline__ void pair_sync() {
+  if constexpr (CG == 2) wgtc::cluster_sync();
+  else __syncthreads();
+}
+// One arrival on the leader's copy of `bar`. What it signals for a pair is that
+// TMEM has been read (ordered by tcgen05.wait and the fences), so it needs no
+// release at cluster scope, which costs about a thousand clocks.
+template <int CG>
+__device__ __forceinline__ void leader_arrive(uint64_t *bar) {
+  if constexpr (CG == 2)
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(wgtc::mapa_shared(wgtc::smem_addr(bar), 0))
+                 : "memory");
+  else mbar_arrive(bar);
+}
+// `bar` of every CTA of the pair receives one arrival when the MMAs issued so far complete.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  if constexpr (CG == 2) wgtc::mma_commit_pair(bar, 3);
+  else wgtc::mma_commit(bar);
+}
+// Tile loads counted on the leader's barrier; `lead` is its shared::cluster
+// address (leader_addr) for a pair.
+template <int CG>
+__device__ __forceinline__ uint32_t leader_addr(uint64_t *bar) {
+  if constexpr (CG == 2) return wgtc::mapa_shared(wgtc::smem_addr(bar), 0);
+  else return wgtc::smem_addr(bar);
+}
+template <int CG>
+__device__ __forceinline__ void load_2d(void *dst, const CUtensorMap *map, uint64_t *bar, uint32_t lead, int c0, int c1) {
+  if constexpr (CG == 2) wgtc::tma_load_2d_pair(dst, map, lead, c0, c1);
+  else wgtc::tma_load_2d(dst, map, bar, c0, c1);
+}
+template <int CG>
+__device__ __forceinline__ void load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, uint32_t lead, int c0, int c1,
+                                        int c2) {
+  if constexpr (CG == 2) wgtc::tma_load_3d_pair(dst, map, lead, c0, c1, c2);
+  else wgtc::tma_load_3d(dst, map, bar, c0, c1, c2);
+}
+template <int CG>
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t *slot, uint32_t cols) {
+  if constexpr (CG == 2) {
+    wgtc::tmem_alloc_pair(slot, cols);
+    wgtc::tmem_relinquish_pair();
+  } else {
+    wgtc::tmem_alloc(slot, cols);
+    wgtc::tmem_relinquish();
+  }
+}
+template <int CG>
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (CG == 2) wgtc::tmem_dealloc_pair(taddr, cols);
+  else wgtc::tmem_dealloc(taddr, cols);
 }
 
 // ---- host side ------------------------------------------------------------
@@ -168,6 +291,26 @@ inline wg_status check_arch(const wg_device *d) {
                    "device %d (%s, sm_%d%d) is not a Blackwell sm_100 device; this library is built "
                    "for sm_100a only", d->ordinal, d->name, d->cc_major, d->cc_minor);
   return WG_OK;
+}
+
+// Launches a kernel over clusters of CG CTAs with programmatic stream
+// serialization (the kernel calls wg_pdl_wait before it touches memory).
+template <int CG, class... KArgs, class... Args>
+cudaError_t launch(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, Args &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Args &&>(args)...);
 }
 
 }  // namespace wgg

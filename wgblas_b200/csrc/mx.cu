@@ -510,7 +510,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
 #pragma unroll
           for (int j = 0; j < 32; j++) r[j] = 0;
         }
-        if (l < a.n) wgg::store_cols<32>(a.C, a.ctype, at + (int64_t)c * a.ldc, a.ldc, x.nv - c, a.alpha, a.beta, r);
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
+        if (l < a.n) wgg::store_cols<32>(a.C, a.ctype, at + (int64_t)c * a.ldc, a.ldc, x.nv - c, a.alpha, a.beta, f);
       }
       wgtc::tc_fence_before();
       mbar_arrive(&acc_empty[b]);
