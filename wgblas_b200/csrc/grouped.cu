@@ -199,7 +199,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   int *start = reinterpret_cast<int *>(smem + S::tables);
   int *tile0 = start + a.groups + 1;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = wgg::warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = wgg::pair_rank<CG>();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
@@ -237,61 +237,61 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   };
 
   if (warp == 0 || warp == 10) {
-    if (lane == 0) {
-      // ---- producers: each CTA of a pair loads its own lanes and its half of the columns ----
-      wgg::Ring<STAGES> ring;
-      bool ok = true;
-      const bool l_side = warp == 0;
-      const uint32_t lead = wgg::leader_addr<CG>(full);
-      for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-        const Tile x = tile_at<MODE, S>(a, t, start, tile0);
-        const int half = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
-        // The first box's outer coordinate, and how many boxes.
-        const int c0 = l_side ? x.l0 + (int)rank * BL : (N_MN ? x.n0 : x.r0) + (int)rank * half;
-        const int boxes = l_side ? 2 : (half + NBOX - 1) / NBOX;
-        const uint32_t bytes = (uint32_t)(l_side ? S::L_BYTES : boxes * NBOX * 128);
-        const int lg = x.g * a.l_group;
-        for (int kb = 0; kb < x.kt; kb++, ring.next()) {
-          const int s = ring.s;
-          ok = wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET);
-          if (!ok) {
-            gave_up(WG_DERR_TMA_WAIT);
-            break;
-          }
-          uint8_t *dst = smem + (size_t)s * S::STAGE + (l_side ? 0 : S::L_BYTES);
-          const int k0 = (MODE == INNER ? x.r0 : 0) + kb * BK;
+    // ---- producers: each CTA of a pair loads its own lanes and its half of the columns ----
+    wgg::Ring<STAGES> ring;
+    bool ok = true;
+    const bool l_side = warp == 0;
+    const uint32_t lead = wgg::leader_addr<CG>(full);
+    for (int64_t t = t_first; t < tiles && ok; t += t_step) {
+      const Tile x = tile_at<MODE, S>(a, t, start, tile0);
+      const int half = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
+      // The first box's outer coordinate, and how many boxes.
+      const int c0 = l_side ? x.l0 + (int)rank * BL : (N_MN ? x.n0 : x.r0) + (int)rank * half;
+      const int boxes = l_side ? 2 : (half + NBOX - 1) / NBOX;
+      const uint32_t bytes = (uint32_t)(l_side ? S::L_BYTES : boxes * NBOX * 128);
+      const int lg = x.g * a.l_group;
+      for (int kb = 0; kb < x.kt; kb++, ring.next()) {
+        const int s = ring.s;
+        ok = wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t *dst = smem + (size_t)s * S::STAGE + (l_side ? 0 : S::L_BYTES);
+        const int k0 = (MODE == INNER ? x.r0 : 0) + kb * BK;
+        const uint32_t at = lead + 8u * (uint32_t)s;
+        if (wgg::elect()) {
           if (MODE == INNER && x.klen - kb * BK < BK && (x.klen & 15)) {
             // A ragged end goes by way of warp 11.
             wgtc::mbar_arrive_expect_tx(&tail[s], bytes);
             for (int b = 0; b < boxes; b++)
               wgtc::tma_load_2d(dst + b * CHUNK, l_side ? &map_l : &map_n, &tail[s], c0 + b * 64, k0);
-            continue;
-          }
-          if (rank == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
-          const uint32_t at = lead + 8u * (uint32_t)s;
-          if (l_side) {
-            if (MODE == ROWS_T) {
-              wgg::load_3d<CG>(dst, &map_l, &full[s], at, k0, c0, lg);
-            } else if (MODE == ROWS_N) {
-              wgg::load_3d<CG>(dst, &map_l, &full[s], at, c0, k0, lg);
-              wgg::load_3d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0, lg);
-            } else {
-              wgg::load_2d<CG>(dst, &map_l, &full[s], at, c0, k0);
-              wgg::load_2d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0);
-            }
           } else {
-            for (int b = 0; b < boxes; b++) {
-              if (N_MN) wgg::load_2d<CG>(dst + b * CHUNK, &map_n, &full[s], at, c0 + b * 64, k0);
-              else wgg::load_2d<CG>(dst + b * NBOX * 128, &map_n, &full[s], at, k0, c0 + b * NBOX);
+            if (rank == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
+            if (l_side) {
+              if (MODE == ROWS_T) {
+                wgg::load_3d<CG>(dst, &map_l, &full[s], at, k0, c0, lg);
+              } else if (MODE == ROWS_N) {
+                wgg::load_3d<CG>(dst, &map_l, &full[s], at, c0, k0, lg);
+                wgg::load_3d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0, lg);
+              } else {
+                wgg::load_2d<CG>(dst, &map_l, &full[s], at, c0, k0);
+                wgg::load_2d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0);
+              }
+            } else {
+              for (int b = 0; b < boxes; b++) {
+                if (N_MN) wgg::load_2d<CG>(dst + b * CHUNK, &map_n, &full[s], at, c0 + b * 64, k0);
+                else wgg::load_2d<CG>(dst + b * NBOX * 128, &map_n, &full[s], at, k0, c0 + b * NBOX);
+              }
             }
           }
         }
+        __syncwarp();
       }
-      // Let every copy (of both CTAs) land before the CTA can exit: the MMAs that
-      // read a stage complete after its copies, and free it.
-      for (int i = 0; i < STAGES && ok; i++, ring.next())
-        if (!wgtc::mbar_wait_bounded(&empty[ring.s], ring.round ^ 1u, WAIT_BUDGET)) break;
     }
+    if (!ok && lane == 0) gave_up(WG_DERR_TMA_WAIT);
+    // Let every copy (of both CTAs) land before the CTA can exit: the MMAs that
+    // read a stage complete after its copies, and free it.
+    for (int i = 0; i < STAGES && ok; i++, ring.next())
+      if (!wgtc::mbar_wait_bounded(&empty[ring.s], ring.round ^ 1u, WAIT_BUDGET)) break;
   } else if (MODE == INNER && warp == 11) {
     // ---- ragged ends: zeroes the lines past a group's last row, then hands the stage on ----
     int s = 0;
@@ -324,7 +324,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       if (++s == STAGES) s = 0;
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---- MMA issuer ----
       wgg::Ring<STAGES> ring;
       int used = 0;
@@ -341,28 +341,32 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         for (int kb0 = 0; kb0 < x.kt && ok; kb0 += segment, used++) {
           const int b = used & 1, kb1 = min(x.kt, kb0 + segment);
           const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
-          ok = wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET);
+          ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET));
           wgtc::tc_fence_after();
-          uint32_t more = 0;
           for (int kb = kb0; kb < kb1 && ok; kb++, ring.next()) {
-            ok = wgtc::mbar_wait_bounded(&full[ring.s], ring.round, WAIT_BUDGET);
+            ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&full[ring.s], ring.round, WAIT_BUDGET));
             if (!ok) break;
             wgtc::tc_fence_after();
             const uint64_t at = (uint64_t)((uint32_t)ring.s * (S::STAGE >> 4));
             const uint64_t dl = desc_l0 + at, dn = desc_n0 + at;
             const int steps = (x.klen - kb * BK + 15) >> 4;
+            if (wgg::elect()) {
+              if (steps >= 4) {
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-              if (kk < steps) {
-                mma_f16<CG>(d_tmem, dl + kk * step_l, dn + kk * step_n, idesc, more);
-                more = 1;
+                for (int kk = 0; kk < 4; kk++)
+                  mma_f16<CG>(d_tmem, dl + kk * step_l, dn + kk * step_n, idesc, kk > 0 || kb > kb0 ? 1u : 0u);
+              } else {
+                for (int kk = 0; kk < steps; kk++)
+                  mma_f16<CG>(d_tmem, dl + kk * step_l, dn + kk * step_n, idesc, kk > 0 || kb > kb0 ? 1u : 0u);
               }
-            wgg::commit<CG>(&empty[ring.s]);
+              wgg::commit<CG>(&empty[ring.s]);
+              if (kb == kb1 - 1) wgg::commit<CG>(&acc_full[b]);
+            }
+            __syncwarp();
           }
-          if (ok) wgg::commit<CG>(&acc_full[b]);
         }
       }
-      if (!ok) gave_up(WG_DERR_MMA_WAIT);
+      if (!ok && lane == 0) gave_up(WG_DERR_MMA_WAIT);
     }
   } else if (warp >= 2 && warp < 2 + EPI_WARPS) {
     // ---- epilogue ----

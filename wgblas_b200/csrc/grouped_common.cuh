@@ -104,6 +104,17 @@ __device__ __forceinline__ int group_of(const int *tile0, int groups, int q) {
   return lo;
 }
 
+// True on one lane of a converged warp. The loops that issue copies and MMAs run
+// on all lanes, with only the instruction itself under elect(): their operands
+// then stay in uniform registers. Issued from a one-lane branch instead, a
+// k-block's four MMAs and commit took 449 clocks instead of 215.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(wgtc::smem_addr(bar)) : "memory");
 }
