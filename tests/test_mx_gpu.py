@@ -178,6 +178,18 @@ def test_gemm(wg, device, m, n, k, ctype):
         x.destroy()
 
 
+@pytest.mark.parametrize("m,n,k", [(2560, 2048, 128), (2570, 2050, 330), (1300, 4100, 1024), (700, 9700, 200),
+                                   (150, 20000, 96)])
+@pytest.mark.parametrize("ctype", ["float32", "bfloat16"])
+def test_gemm_pairs(wg, device, m, n, k, ctype):
+    test_gemm(wg, device, m, n, k, ctype)
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 130, 9000), (2570, 2050, 4500)])
+def test_gemm_long(wg, device, m, n, k):
+    test_gemm(wg, device, m, n, k, "float32")
+
+
 @pytest.mark.parametrize("ctype", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("alpha,beta", [(0.5, 1.0), (-2.0, 0.25), (0.0, 0.0), (0.0, -1.5), (0.0, 1.0)])
 def test_gemm_scalars(wg, device, ctype, alpha, beta):
@@ -240,3 +252,8 @@ def test_gemm_grouped(wg, device, sizes, first, after, n, k):
     gc.assert_close(values(wg, C).reshape(m, n), want, mag, k, 0.5, c0.astype(np.float64), "float32", "C")
     for x in (a, b, W, C, off):
         x.destroy()
+
+
+@pytest.mark.parametrize("n,k", [(2048, 128), (2050, 600)])
+def test_gemm_grouped_pairs(wg, device, n, k):
+    test_gemm_grouped(wg, device, [150, 0, 1, 290, 256, 257, 31, 140, 513, 160, 64, 130, 129, 200, 300], 1, 5, n, k)

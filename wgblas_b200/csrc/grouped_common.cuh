@@ -194,6 +194,14 @@ __device__ __forceinline__ void store_sums(float *at, int64_t ldc, int valid, fl
     if (c < valid) store_typed<float, 16>(at, ldc, valid - c, alpha, beta, sum + c, [](float x) { return x; });
 }
 
+template <int CPT>
+__device__ __forceinline__ void store_all(void *C, int type, int64_t at, int64_t ldc, int valid, float alpha,
+                                          float beta, const float (&sum)[CPT]) {
+#pragma unroll
+  for (int c = 0; c < CPT; c += 16)
+    if (c < valid) store_cols<16>(C, type, at + (int64_t)c * ldc, ldc, valid - c, alpha, beta, sum + c);
+}
+
 // Stores CPT accumulator columns straight from TMEM (`from` false: zeros instead).
 template <int CPT>
 __device__ __forceinline__ void store_acc(uint32_t taddr, bool from, void *C, int type, int64_t at, int64_t ldc,

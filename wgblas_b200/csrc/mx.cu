@@ -265,38 +265,48 @@ __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
 //
 // The grouped kernel's frame and roles (grouped.cu): B's rows on the lanes, A's
 // rows on the columns, both K-major. A k-block is 256 elements, 128 bytes of
-// codes a row and two scale tiles of 128 rows for each operand; the MMA warp
+// codes a row and two scale tiles for each 128 rows of an operand; the MMA warp
 // copies the scale tiles to TMEM (tcgen05.cp, four columns a tile) in front of
 // the block's four MMAs of 64.
+//
+// Forms: CTA pairs with 256 x 256 tiles for compute-bound calls (an MMA of 64
+// takes as long as a bf16 one of 16, so the bytes a tile needs from L2 a clock
+// are the same as there, and with them the reason for pairs), one CTA with
+// 128 x 128 tiles otherwise. A pair's accumulator and scales leave no room for a
+// second accumulator in TMEM: the epilogue drains it to registers at once and
+// stores from there while the next tile's MMAs run.
 
 constexpr int BKE = 256;           // elements of a k-block
-constexpr int EPI_WARPS = 4;
+constexpr int EPI_WARPS = wgg::EPI_WARPS;
 constexpr size_t SMEM_LIMIT = 227 * 1024;
+// fp32 results: k-blocks between drains of the accumulator, whose additions
+// truncate (grouped.cu).
+constexpr int SEG = 16;
 
-template <int BN_>
+template <int CG_, int BN_>
 struct Shape {
-  static constexpr int BN = BN_;
-  static constexpr int NT = BN / 128;            // scale tiles of the N side
-  static constexpr int L_BYTES = BL * 128, N_BYTES = BN * 128;
+  static constexpr int CG = CG_, BN = BN_;
+  static constexpr int TL = CG * BL, CPT = BN / 2;
+  static constexpr int NT = BN / 128;            // scale tiles of the N side (every CTA of a pair has all)
+  static constexpr int L_BYTES = BL * 128, N_BYTES = BN / CG * 128;
   static constexpr int SF_L = 1024, SF_N = NT * 1024;
   static constexpr int STAGE = L_BYTES + N_BYTES + SF_L + SF_N;
-  static constexpr int STAGES = (int)((SMEM_LIMIT - 12 * 1024) / STAGE);
+  static constexpr int STAGES = (int)((SMEM_LIMIT - 14 * 1024) / STAGE);
   // TMEM columns: accumulators, then two sets of scales (L: 2 x 4, N: 2 x 4 NT).
   static constexpr int ACCS = BN <= 128 ? 2 : 1;
   static constexpr int SF_COL = ACCS * BN, SF_SET = 8 + 8 * NT;
   static constexpr int TMEM_COLS = 512;
   static_assert(SF_COL + 2 * SF_SET <= TMEM_COLS, "accumulators and scales must fit TMEM");
-  static constexpr size_t smem(int groups) {
-    return 1024 + (size_t)STAGES * STAGE + 256 + 3 * ((size_t)groups + 1) * sizeof(int);
-  }
+  static constexpr size_t tables = (size_t)STAGES * STAGE + 256;
+  static constexpr size_t smem(int groups) { return 1024 + tables + 3 * ((size_t)groups + 1) * sizeof(int); }
+  static constexpr int NMMA_STEP = 32;
 };
 
 struct Args {
   int groups, rows, n, k;
-  int tiles_l, katoms;
+  int tiles_l;
   int l_atoms;           // scale tile rows of one matrix of B
   const int *offsets;    // NULL: one group, all rows
-  const uint8_t *sf_l, *sf_n;
   float alpha, beta;
   void *C;
   int64_t ldc;
@@ -313,30 +323,37 @@ __device__ __forceinline__ uint32_t idesc_mxf4(int M, int N, uint32_t sf_id) {
          (sf_id << 29) | (sf_id << 4);
 }
 
+template <int CG>
 __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
 
-// Copies one 512-byte scale tile (32 lines of 16 bytes) to four TMEM columns of
-// every lane quarter.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
-  // no swizzle, 8-line groups 128 bytes apart
-  const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// Copies one 512-byte scale tile (32 lines of 16 bytes, no swizzle, eight-line
+// groups 128 bytes apart) to four TMEM columns of every lane quarter; for a pair,
+// each CTA from its own shared memory to its own TMEM.
+__device__ __forceinline__ uint64_t scales_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
 }
-
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          wgtc::smem_addr(dst)),
-      "l"(src), "r"(bytes), "r"(wgtc::smem_addr(bar))
-      : "memory");
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 struct Tile {
@@ -352,7 +369,7 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
   x.g = wgg::group_of(tile0, a.groups, q);
   const int ntok = tile0[x.g + 1] - tile0[x.g];
   const int local = (int)(t - (int64_t)tile0[x.g] * a.tiles_l);
-  x.l0 = (local / ntok) * BL;
+  x.l0 = (local / ntok) * S::TL;
   const int first = (local % ntok) * S::BN;
   x.r0 = start[x.g] + first;
   x.nv = min(S::BN, start[x.g + 1] - x.r0);
@@ -360,10 +377,13 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
   return x;
 }
 
-template <class S>
-__global__ void __launch_bounds__(192, 1)
-mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n, const Args a) {
-  constexpr int STAGES = S::STAGES;
+// Warps: 0 and 10 load (the L and the N side, codes and scales), 1 issues the
+// MMAs, 2-9 store. SUMS: the accumulator is drained every SEG k-blocks.
+template <class S, bool SUMS>
+__global__ void __launch_bounds__(352, 1)
+mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n,
+               const __grid_constant__ CUtensorMap map_sl, const __grid_constant__ CUtensorMap map_sn, const Args a) {
+  constexpr int STAGES = S::STAGES, CG = S::CG;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = wgtc::smem_addr(smem_raw);
   uint8_t *smem = smem_raw + ((1024 - (base & 1023)) & 1023);
@@ -373,159 +393,179 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   uint64_t *acc_empty = acc_full + 2;   // [2]
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  int *start = reinterpret_cast<int *>(smem + (size_t)STAGES * S::STAGE + 256);
+  int *start = reinterpret_cast<int *>(smem + S::tables);
   int *tile0 = start + a.groups + 1, *atom0 = tile0 + a.groups + 1;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = wgg::warp_index(), lane = threadIdx.x & 31;
+  const uint32_t rank = wgg::pair_rank<CG>();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
-      wgtc::mbar_init(&full[s], 1);
+      wgtc::mbar_init(&full[s], 2);
       wgtc::mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       wgtc::mbar_init(&acc_full[b], 1);
-      wgtc::mbar_init(&acc_empty[b], 32 * EPI_WARPS);
+      wgtc::mbar_init(&acc_empty[b], CG * EPI_WARPS);
     }
     *abort_flag = 0;
     wgtc::fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
     wgtc::prefetch_tensormap(&map_l);
+    wgtc::prefetch_tensormap(&map_sl);
+  }
+  if (warp == 10 && lane == 0) {
     wgtc::prefetch_tensormap(&map_n);
+    wgtc::prefetch_tensormap(&map_sn);
   }
-  if (warp == 1) {
-    wgtc::tmem_alloc(tmem_slot, S::TMEM_COLS);
-    wgtc::tmem_relinquish();
-  }
+  if (warp == 1) wgg::pair_tmem_alloc<CG>(tmem_slot, S::TMEM_COLS);
   wg_pdl_wait();
   wg_pdl_trigger();
   wgg::plan_groups(a.offsets, a.groups, a.rows, S::BN, start, tile0, atom0, a.dwords);
   wgtc::tc_fence_before();
-  __syncthreads();
+  wgg::pair_sync<CG>();
   wgtc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int64_t tiles = (int64_t)tile0[a.groups] * a.tiles_l;
+  const int64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
   const int kt = a.alpha == 0.0f ? 0 : (a.k + BKE - 1) / BKE;
+  auto gave_up = [&](unsigned bit) {
+    atomicOr(a.dwords + WG_DW_ERROR, bit);
+    *abort_flag = 1;
+  };
 
-  if (warp == 0 && lane == 0) {
-    // ---- producer: codes by TMA, scale tiles by bulk copies ----
-    int64_t it = 0;
+  if (warp == 0 || warp == 10) {
+    // ---- producers ----
+    wgg::Ring<STAGES> ring;
     bool ok = true;
-    for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    const bool l_side = warp == 0;
+    const uint32_t lead = wgg::leader_addr<CG>(full);
+    for (int64_t t = t_first; t < tiles && ok; t += t_step) {
       const Tile x = tile_at<S>(a, t, start, tile0, atom0);
-      const int boxes = (x.nv + 63) / 64, atoms = (x.nv + 127) / 128;
-      const uint8_t *sl = a.sf_l + ((int64_t)x.g * a.l_atoms + x.l0 / 128) * a.katoms * 512;
-      const uint8_t *sn = a.sf_n + (int64_t)x.n_atom * a.katoms * 512;
-      for (int kb = 0; kb < kt; kb++, it++) {
-        const int s = (int)(it % STAGES);
-        if (!wgtc::mbar_wait_bounded(&empty[s], ((uint32_t)(it / STAGES) & 1u) ^ 1u, WAIT_BUDGET) || *abort_flag) {
-          atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_TMA_WAIT);
-          *abort_flag = 1;
-          ok = false;
-          break;
+      const int half = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
+      const int boxes = (half + 63) / 64;
+      const int l0 = x.l0 + (int)rank * BL, r0 = x.r0 + (int)rank * half;
+      const int sl = x.g * a.l_atoms + l0 / 128;
+      const uint32_t bytes = l_side ? (uint32_t)(S::L_BYTES + S::SF_L) : (uint32_t)(boxes * 8192 + S::SF_N);
+      for (int kb = 0; kb < kt; kb++, ring.next()) {
+        const int s = ring.s;
+        ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET));
+        if (!ok) break;
+        uint8_t *st = smem + (size_t)s * S::STAGE, *sf = st + S::L_BYTES + S::N_BYTES;
+        const uint32_t at = lead + 8u * (uint32_t)s;
+        if (wgg::elect()) {
+          if (rank == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
+          // (what lies past the last scale tile, or past the matrix's rows, arrives as zeros)
+          if (l_side) {
+            wgg::load_3d<CG>(st, &map_l, &full[s], at, kb * 128, l0, x.g);
+            wgg::load_2d<CG>(sf, &map_sl, &full[s], at, kb * 256, sl);
+          } else {
+            for (int b = 0; b < boxes; b++)
+              wgg::load_2d<CG>(st + S::L_BYTES + b * 8192, &map_n, &full[s], at, kb * 128, r0 + b * 64);
+            wgg::load_2d<CG>(sf + S::SF_L, &map_sn, &full[s], at, kb * 256, x.n_atom);
+          }
         }
-        uint8_t *st = smem + (size_t)s * S::STAGE;
-        // The last k-block may have one scale tile instead of two.
-        const uint32_t sf = (uint32_t)min(2, a.katoms - kb * 2) * 512u;
-        wgtc::mbar_arrive_expect_tx(&full[s], (uint32_t)(S::L_BYTES + boxes * 64 * 128) + sf * (1 + atoms));
-        wgtc::tma_load_3d(st, &map_l, &full[s], kb * 128, x.l0, x.g);
-        for (int b = 0; b < boxes; b++)
-          wgtc::tma_load_2d(st + S::L_BYTES + b * 8192, &map_n, &full[s], kb * 128, x.r0 + b * 64);
-        uint8_t *sf_at = st + S::L_BYTES + S::N_BYTES;
-        bulk_load(sf_at, sl + kb * 1024, sf, &full[s]);
-        for (int b = 0; b < atoms; b++)
-          bulk_load(sf_at + 1024 * (1 + b), sn + ((int64_t)b * a.katoms + kb * 2) * 512, sf, &full[s]);
+        __syncwarp();
       }
     }
-    for (int64_t q = it - STAGES > 0 ? it - STAGES : 0; q < it; q++)
-      wgtc::mbar_wait_bounded(&full[q % STAGES], (uint32_t)(q / STAGES) & 1u, WAIT_BUDGET);
-  } else if (warp == 1 && lane == 0) {
-    // ---- MMA issuer ----
-    int64_t it = 0;
-    int used = 0;
-    bool ok = true;
-    for (int64_t t = blockIdx.x; t < tiles && ok && kt; t += gridDim.x, used++) {
-      const Tile x = tile_at<S>(a, t, start, tile0, atom0);
-      const int nmma = (x.nv + 31) & ~31, atoms = (x.nv + 127) / 128;
-      const int b = used % S::ACCS;
-      if (!wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used / S::ACCS) & 1u) ^ 1u, WAIT_BUDGET) || *abort_flag) {
-        atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_MMA_WAIT);
-        *abort_flag = 1;
-        break;
-      }
-      wgtc::tc_fence_after();
-      const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
-      for (int kb = 0; kb < kt; kb++, it++) {
-        const int s = (int)(it % STAGES);
-        if (!wgtc::mbar_wait_bounded(&full[s], (uint32_t)(it / STAGES) & 1u, WAIT_BUDGET) || *abort_flag) {
-          atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_TMA_WAIT);
-          *abort_flag = 1;
-          ok = false;
-          break;
+    if (!ok && lane == 0) gave_up(WG_DERR_TMA_WAIT);
+    // Let every copy (of both CTAs) land before the CTA can exit.
+    for (int i = 0; i < STAGES && ok; i++, ring.next())
+      if (!wgtc::mbar_wait_bounded(&empty[ring.s], ring.round ^ 1u, WAIT_BUDGET)) break;
+  } else if (warp == 1) {
+    if (rank == 0) {
+      // ---- MMA issuer ----
+      wgg::Ring<STAGES> ring;
+      int used = 0;
+      uint32_t set = 0;  // which set of scale columns
+      constexpr int segment = SUMS ? SEG : 1 << 30;
+      const uint32_t smem0 = wgtc::smem_addr(smem);
+      const uint64_t desc_l0 = wgtc::smem_desc_kmajor(smem0, 128);
+      const uint64_t desc_n0 = wgtc::smem_desc_kmajor(smem0 + S::L_BYTES, 128);
+      const uint64_t desc_s0 = scales_desc(smem0 + S::L_BYTES + S::N_BYTES);
+      bool ok = true;
+      for (int64_t t = t_first; t < tiles && ok; t += t_step) {
+        const Tile x = tile_at<S>(a, t, start, tile0, atom0);
+        const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
+        const uint32_t idesc0 = idesc_mxf4(S::TL, nmma, 0), idesc2 = idesc_mxf4(S::TL, nmma, 2);
+        for (int kb0 = 0; kb0 < kt && ok; kb0 += segment, used++) {
+          const int b = used % S::ACCS, kb1 = min(kt, kb0 + segment);
+          const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
+          ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used / S::ACCS) & 1u) ^ 1u, WAIT_BUDGET));
+          wgtc::tc_fence_after();
+          for (int kb = kb0; kb < kb1 && ok; kb++, ring.next(), set ^= 1u) {
+            ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&full[ring.s], ring.round, WAIT_BUDGET));
+            if (!ok) break;
+            wgtc::tc_fence_after();
+            const uint64_t at = (uint64_t)((uint32_t)ring.s * (S::STAGE >> 4));
+            const uint64_t dl = desc_l0 + at, dn = desc_n0 + at, ds = desc_s0 + at;
+            const uint32_t tl = tmem + S::SF_COL + set * S::SF_SET, tn = tl + 8;
+            const int steps = (a.k - kb * BKE + 63) >> 6;
+            if (wgg::elect()) {
+#pragma unroll
+              for (int j = 0; j < 2; j++) {
+                copy_scales<CG>(tl + 4 * j, ds + 32 * j);
+#pragma unroll
+                for (int r = 0; r < S::NT; r++)
+                  copy_scales<CG>(tn + 4 * S::NT * j + 4 * r, ds + 64 * (1 + r) + 32 * j);
+              }
+              if (steps >= 4) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                  mma_mxf4<CG>(d_tmem, dl + i * 2, dn + i * 2, i & 1 ? idesc2 : idesc0, tl + 4 * (i >> 1),
+                               tn + 4 * S::NT * (i >> 1), i > 0 || kb > kb0 ? 1u : 0u);
+              } else {
+                for (int i = 0; i < steps; i++)
+                  mma_mxf4<CG>(d_tmem, dl + i * 2, dn + i * 2, i & 1 ? idesc2 : idesc0, tl + 4 * (i >> 1),
+                               tn + 4 * S::NT * (i >> 1), i > 0 || kb > kb0 ? 1u : 0u);
+              }
+              wgg::commit<CG>(&empty[ring.s]);
+              if (kb == kb1 - 1) wgg::commit<CG>(&acc_full[b]);
+            }
+            __syncwarp();
+          }
         }
-        wgtc::tc_fence_after();
-        const uint32_t st = wgtc::smem_addr(smem + (size_t)s * S::STAGE);
-        const uint32_t sn = st + S::L_BYTES, sf = sn + S::N_BYTES;
-        const uint32_t tl = tmem + S::SF_COL + (uint32_t)(it & 1) * S::SF_SET, tn = tl + 8;
-        const int katoms = min(2, a.katoms - kb * 2);
-        for (int j = 0; j < katoms; j++) {
-          copy_scales(tl + 4 * j, sf + 512 * j);
-          for (int r = 0; r < atoms; r++) copy_scales(tn + 4 * S::NT * j + 4 * r, sf + 1024 * (1 + r) + 512 * j);
-        }
-        const int steps = min(4, (a.k - kb * BKE + 63) / 64);
-        for (int i = 0; i < steps; i++)
-          mma_mxf4(d_tmem, wgtc::smem_desc_kmajor(st + i * 32, 128), wgtc::smem_desc_kmajor(sn + i * 32, 128),
-                   idesc_mxf4(BL, nmma, (uint32_t)(i & 1) * 2), tl + 4 * (i >> 1), tn + 4 * S::NT * (i >> 1),
-                   (kb > 0 || i > 0) ? 1u : 0u);
-        wgtc::mma_commit(&empty[s]);
       }
-      if (ok) wgtc::mma_commit(&acc_full[b]);
+      if (!ok && lane == 0) gave_up(WG_DERR_MMA_WAIT);
     }
-  } else if (warp >= 2) {
+  } else if (warp >= 2 && warp < 2 + EPI_WARPS) {
     // ---- epilogue ----
-    const int q = warp & 3;
+    const int q = warp & 3, h = (warp - 2) >> 2;
     int used = 0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, used++) {
+    bool ok = true;
+    for (int64_t t = t_first; t < tiles && ok; t += t_step) {
       const Tile x = tile_at<S>(a, t, start, tile0, atom0);
-      const int b = used % S::ACCS;
-      if (kt) {
-        bool ready = wgtc::mbar_wait_bounded(&acc_full[b], (uint32_t)(used / S::ACCS) & 1u, WAIT_BUDGET) && *abort_flag == 0;
-        ready = __all_sync(0xffffffffu, ready);
-        if (!ready) {
-          if (lane == 0) atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_MMA_WAIT);
-          *abort_flag = 1;
+      const int valid = x.nv - h * S::CPT;  // columns this warp has (may be none)
+      const int l = x.l0 + (int)rank * BL + q * 32 + lane;
+      const int64_t at = (int64_t)(x.r0 + h * S::CPT) * a.ldc + l;
+      const uint32_t col = tmem + (uint32_t)(h * S::CPT) + ((uint32_t)(q * 32) << 16);
+      float sum[S::CPT];
+#pragma unroll
+      for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
+      for (int kb0 = 0; kb0 < kt; kb0 += SUMS ? SEG : 1 << 30, used++) {
+        const int b = used % S::ACCS;
+        ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_full[b], (uint32_t)(used / S::ACCS) & 1u, WAIT_BUDGET) &&
+                                         *abort_flag == 0);
+        if (!ok) {
+          if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
           break;
         }
         wgtc::tc_fence_after();
+        wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == 0, sum);
+        wgtc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) wgg::leader_arrive<CG>(&acc_empty[b]);
       }
-      const int l = x.l0 + q * 32 + lane;
-      const int64_t at = (int64_t)x.r0 * a.ldc + l;
-      const uint32_t trow = tmem + (uint32_t)(b * S::BN) + ((uint32_t)(q * 32) << 16);
-      for (int c = 0; c < x.nv; c += 32) {
-        uint32_t r[32];
-        if (kt) {
-          wgtc::tmem_ld_32x32b_x32(trow + (uint32_t)c, r);
-          wgtc::tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j++) r[j] = 0;
-        }
-        float f[32];
-#pragma unroll
-        for (int j = 0; j < 32; j++) f[j] = __uint_as_float(r[j]);
-        if (l < a.n) wgg::store_cols<32>(a.C, a.ctype, at + (int64_t)c * a.ldc, a.ldc, x.nv - c, a.alpha, a.beta, f);
-      }
-      wgtc::tc_fence_before();
-      mbar_arrive(&acc_empty[b]);
+      if (ok && l < a.n) wgg::store_all<S::CPT>(a.C, a.ctype, at, a.ldc, valid, a.alpha, a.beta, sum);
     }
   }
 
   wgtc::tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  wgg::pair_sync<CG>();
   if (warp == 1) {
-    __syncwarp();
     wgtc::tc_fence_after();
-    wgtc::tmem_dealloc(tmem, S::TMEM_COLS);
+    wgg::pair_tmem_dealloc<CG>(tmem, S::TMEM_COLS);
   }
 }
 
@@ -569,38 +609,54 @@ wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const Quan
   return WG_OK;
 }
 
-bool encode(CUtensorMap *map, const void *ptr, int rank, const cuuint64_t *dims, const cuuint64_t *strides,
-            const cuuint32_t *box) {
+bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *ptr, int rank, const cuuint64_t *dims,
+            const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle) {
   wg_encode_tiled_fn fn = wg_encode_tiled();
   if (!fn) return false;
   const cuuint32_t estr[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void *>(ptr), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, type, rank, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Operands {
+  const uint8_t *A, *As, *B, *Bs;
+};
+
+template <class S, bool SUMS>
+wg_status launch_as(wg_device *d, const char *family, Args &a, const CUtensorMap (&m)[4]) {
+  const int64_t most = ((int64_t)a.rows / S::BN + a.groups) * a.tiles_l;
+  const unsigned grid = S::CG * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CG));
+  wg_launch_scope scope(d, family);
+  WG_CUDA(wg_kernel_smem(mx_gemm_kernel<S, SUMS>, SMEM_LIMIT));
+  WG_CUDA((wgg::launch<S::CG>(mx_gemm_kernel<S, SUMS>, grid, 352, S::smem(a.groups), d->stream, m[0], m[1], m[2], m[3], a)));
+  WG_CUDA(cudaGetLastError());
+  return WG_OK;
 }
 
 template <class S>
-wg_status launch_gemm(wg_device *d, const char *family, const Args &a, const uint8_t *A, const uint8_t *B) {
-  CUtensorMap ml, mn;
-  memset(&ml, 0, sizeof ml);
-  memset(&mn, 0, sizeof mn);
+wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands &o) {
+  CUtensorMap m[4];
+  memset(m, 0, sizeof m);
+  a.tiles_l = (a.n + S::TL - 1) / S::TL;
   if (a.alpha != 0.0f) {
-    const cuuint64_t pitch = (cuuint64_t)pitch_of(a.k);
-    const cuuint64_t dl[3] = {pitch, (cuuint64_t)a.n, (cuuint64_t)a.groups};
-    const cuuint64_t sl[2] = {pitch, pitch * (cuuint64_t)a.n};
+    const cuuint64_t pitch = (cuuint64_t)pitch_of(a.k), words = (cuuint64_t)tiles_of(a.k) * 128;
+    const cuuint64_t dl[3] = {pitch, (cuuint64_t)a.n, (cuuint64_t)a.groups}, sl[2] = {pitch, pitch * (cuuint64_t)a.n};
     const cuuint32_t bl[3] = {128, (cuuint32_t)BL, 1};
     const cuuint64_t dn[2] = {pitch, (cuuint64_t)a.rows};
     const cuuint32_t bn[2] = {128, 64};
-    if (!encode(&ml, B, 3, dl, sl, bl) || !encode(&mn, A, 2, dn, sl, bn))
+    // Scales: rows of tiles, as 32-bit words; a box is two tiles long.
+    const cuuint64_t ss = words * 4;
+    const cuuint64_t dsl[2] = {words, (cuuint64_t)a.l_atoms * (cuuint64_t)a.groups};
+    const cuuint64_t dsn[2] = {words, (cuuint64_t)tiles_of(a.rows) + (a.offsets ? (cuuint64_t)a.groups : 0)};
+    const cuuint32_t bsl[2] = {256, 1}, bsn[2] = {256, (cuuint32_t)S::NT};
+    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
+    const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B, no = CU_TENSOR_MAP_SWIZZLE_NONE;
+    if (!encode(&m[0], u8, o.B, 3, dl, sl, bl, sw) || !encode(&m[1], u8, o.A, 2, dn, sl, bn, sw) ||
+        !encode(&m[2], u32, o.Bs, 2, dsl, &ss, bsl, no) || !encode(&m[3], u32, o.As, 2, dsn, &ss, bsn, no))
       return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
   }
-  const int64_t most = ((int64_t)a.rows / S::BN + a.groups) * a.tiles_l;
-  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count));
-  wg_launch_scope scope(d, family);
-  WG_CUDA(wg_kernel_smem(mx_gemm_kernel<S>, SMEM_LIMIT));
-  WG_CUDA(wg_launch_pdl(mx_gemm_kernel<S>, dim3(grid), dim3(192), S::smem(a.groups), d->stream, ml, mn, a));
-  WG_CUDA(cudaGetLastError());
-  return WG_OK;
+  return a.ctype == WG_TYPE_F32 && a.k > SEG * BKE ? launch_as<S, true>(d, family, a, m)
+                                                   : launch_as<S, false>(d, family, a, m);
 }
 
 wg_status mx_gemm(wg_device *d, const char *family, int ctype, int64_t groups, int64_t m, int64_t n, int64_t k,
@@ -633,22 +689,20 @@ wg_status mx_gemm(wg_device *d, const char *family, int ctype, int64_t groups, i
   a.rows = (int)m;
   a.n = (int)n;
   a.k = (int)k;
-  a.tiles_l = (int)tiles_of(n);
-  a.katoms = (int)tiles_of(k);
   a.l_atoms = (int)tiles_of(n);
   a.offsets = offsets;
-  a.sf_l = static_cast<const uint8_t *>(Bs);
-  a.sf_n = static_cast<const uint8_t *>(As);
   a.alpha = alpha;
   a.beta = beta;
   a.C = C;
   a.ldc = ldc;
   a.ctype = ctype;
   a.dwords = d->dwords;
-  const uint8_t *pa = static_cast<const uint8_t *>(A), *pb = static_cast<const uint8_t *>(B);
+  const Operands o = {static_cast<const uint8_t *>(A), static_cast<const uint8_t *>(As),
+                      static_cast<const uint8_t *>(B), static_cast<const uint8_t *>(Bs)};
   return wg_timed(d, gpu_ms, [&] {
-    return m / groups <= 128 ? launch_gemm<Shape<128>>(d, family, a, pa, pb)
-                             : launch_gemm<Shape<256>>(d, family, a, pa, pb);
+    const int64_t pairs = (n + 255) / 256 * std::max<int64_t>(groups, m / 256);
+    return m / groups > 128 && 2 * pairs >= d->sm_count ? launch_gemm<Shape<2, 256>>(d, family, a, o)
+                                                        : launch_gemm<Shape<1, 128>>(d, family, a, o);
   });
 }
 
