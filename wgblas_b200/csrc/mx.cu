@@ -74,20 +74,29 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-// Eight elements at p of which the first `valid` exist, as float32.
+// Eight elements as they are stored.
 template <class T>
-__device__ __forceinline__ void load8(const T *p, int valid, float (&x)[8]) {
-  if (valid >= 8 && ((uintptr_t)p & 15) == 0) {
-    uint4 w[sizeof(T) / 2];
+union Eight {
+  uint4 w[sizeof(T) / 2];
+  T v[8];
+  __device__ __forceinline__ Eight() {}
+};
+
+// The float32 bits of the largest magnitude of eight elements (a NaN is larger
+// than any number). 16-bit types compare as pairs of integers.
+__device__ __forceinline__ uint32_t top_of(const Eight<float> &w) {
+  uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-    const T *v = reinterpret_cast<const T *>(w);
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = to_float(v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = i < valid ? to_float(p[i]) : 0.0f;
-  }
+  for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(w.v[i]) & 0x7fffffffu);
+  return top;
+}
+template <class T>
+__device__ __forceinline__ uint32_t top_of(const Eight<T> &w) {
+  const uint4 u = w.w[0];
+  const uint32_t m = 0x7fff7fffu;
+  const uint32_t p = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+  const uint16_t h = (uint16_t)max(p & 0xffffu, p >> 16);
+  return __float_as_uint(to_float(*reinterpret_cast<const T *>(&h)));
 }
 
 // The rows of one scale tile: first row, how many, and its matrix (batch).
@@ -116,53 +125,96 @@ __device__ __forceinline__ TileRows rows_of_tile(const QuantArgs &a, int tile, i
   return t;
 }
 
-// One CTA per scale tile (128 rows x 128 columns): 16 threads a row, eight
-// elements each, four threads a block; the tile's scales are gathered in shared
-// memory and written as one piece.
+// Scales of two neighbouring tiles (128 rows x 256 columns) of a tile row,
+// between shared memory and their place.
+__device__ __forceinline__ uint32_t *tile_scales(const QuantArgs &a, int tile, int tc) {
+  return reinterpret_cast<uint32_t *>(a.scales + ((int64_t)tile * a.tiles_c + tc) * 512);
+}
+__device__ __forceinline__ int scale_at(int r, int block) {  // block 0 .. 7 of the two tiles
+  return (block >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (block & 3);
+}
+
+constexpr int ROWS_AT_ONCE = 4;  // a warp's loads in flight
+
+// One CTA per two scale tiles: a warp takes whole 256-column lines, eight
+// elements a thread, four threads a block. Bound by memory: 16-byte loads, four
+// in flight a thread; a line's codes are one 128-byte store, the scales are
+// gathered in shared memory and written as one piece. 8192 x 8192 bf16: see the
+// figures at launch_quant.
 template <class T>
 __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
   extern __shared__ int tables[];
-  __shared__ __align__(16) uint8_t sf[512];
+  __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
-  const int tile = (int)(blockIdx.x / (unsigned)a.tiles_c), tc = (int)(blockIdx.x % (unsigned)a.tiles_c);
+  const int pairs = (a.tiles_c + 1) >> 1;
+  const int tile = (int)(blockIdx.x / (unsigned)pairs), tc = (int)(blockIdx.x % (unsigned)pairs) * 2;
   const TileRows t = rows_of_tile(a, tile, tables);
   if (t.n <= 0) return;
-  if (threadIdx.x < 128) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = 0;
+  reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = 0;
   __syncthreads();
-  const T *X = static_cast<const T *>(a.X) + t.b * a.strideX;
-  const int c = threadIdx.x & 15, col = tc * 128 + c * 8;
+  const int warp = threadIdx.x >> 5, c = threadIdx.x & 31, col = tc * 128 + c * 8;
+  const T *X = static_cast<const T *>(a.X) + t.b * a.strideX + col;
   const bool in = col / 32 * 16 < a.pitch;  // the block exists (it may end in padding)
-  for (int r = threadIdx.x >> 4; r < t.n; r += 16) {
-    const int64_t row = t.r0 + r;
-    float x[8];
-    load8(X + row * a.ldx + col, in ? a.cols - col : 0, x);
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    // The loop's bound differs between rows: name the block's four lanes.
-    const uint32_t four = 0xfu << (threadIdx.x & 28);
-    top = max(top, __shfl_xor_sync(four, top, 1));
-    top = max(top, __shfl_xor_sync(four, top, 2));
+  const int valid = in ? a.cols - col : 0;
+  // (the whole warp takes one way: the lines' shuffles need all its lanes)
+  const bool wide = __all_sync(0xffffffffu, valid >= 8 && ((uintptr_t)X & 15) == 0 && a.ldx * sizeof(T) % 16 == 0);
+  uint8_t *codes = a.codes + (int64_t)t.b * a.rows * a.pitch + col / 2;
+  const T *src = X + (t.r0 + (int64_t)warp) * a.ldx;
+  uint8_t *dst = codes + (t.r0 + (int64_t)warp) * a.pitch;
+  uint8_t *sfb = sf + (c >> 4) * 512 + (c >> 2 & 3);
+  const int64_t src_step = 8 * a.ldx, dst_step = 8 * a.pitch;
+  // Rounds one line's eight elements; `r` is the line within the tile.
+  auto round = [&](const Eight<T> &w, uint8_t *to, int r) {
+    uint32_t top = top_of(w);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t e = scale_byte(top);
     const float inv = inverse_scale(e);
+    float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] *= inv;
+    for (int i = 0; i < 8; i++) x[i] = to_float(w.v[i]) * inv;
     if (in) {
-      const int64_t at = ((int64_t)t.b * a.rows + row) * a.pitch + col / 2;
-      *reinterpret_cast<uint32_t *>(a.codes + at) = encode8(x);
-      if ((c & 3) == 0) sf[(r & 31) * 16 + (r >> 5) * 4 + (c >> 2)] = (uint8_t)e;
+      *reinterpret_cast<uint32_t *>(to) = encode8(x);
+      if ((c & 3) == 0) sfb[(r & 31) * 16 + (r >> 5) * 4] = (uint8_t)e;
+    }
+  };
+  int r = warp;
+  if (wide) {
+    for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
+      Eight<T> w[ROWS_AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step)
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) round(w[u], dst, r + 8 * u);
     }
   }
+  for (; r < t.n; r += 8, src += src_step, dst += dst_step) {
+    Eight<T> w;
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; i++) w.w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) w.v[i] = i < valid ? src[i] : T(0.0f);
+    }
+    round(w, dst, r);
+  }
   __syncthreads();
-  if (threadIdx.x < 32)
-    reinterpret_cast<uint4 *>(a.scales + ((int64_t)tile * a.tiles_c + tc) * 512)[threadIdx.x] =
-        reinterpret_cast<const uint4 *>(sf)[threadIdx.x];
+  // (the second tile exists unless the tile row has an odd number of them)
+  if (threadIdx.x < 128 || tc + 1 < a.tiles_c) tile_scales(a, tile, tc)[threadIdx.x] = reinterpret_cast<const uint32_t *>(sf)[threadIdx.x];
 }
 
-// The transposed form: X holds the matrix's columns as its rows. A thread takes
-// one row of the result and 32 of X's rows; a warp's loads are 32 neighbouring
-// elements.
+// The transposed form: X holds the matrix's columns as its rows. One CTA per
+// scale tile; a thread takes two neighbouring rows of the result and one block
+// of them, 32 of X's lines: its loads are independent, and a warp's are 64
+// neighbouring elements.
+template <class T>
+struct Two {
+  T v[2];
+};
 template <class T>
 __global__ void __launch_bounds__(256) mx_quantize_t(const QuantArgs a) {
   __shared__ __align__(16) uint8_t sf[512];
@@ -172,48 +224,57 @@ __global__ void __launch_bounds__(256) mx_quantize_t(const QuantArgs a) {
   const TileRows t = rows_of_tile(a, tile, nullptr);
   if (threadIdx.x < 128) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = 0;
   __syncthreads();
-  const T *X = static_cast<const T *>(a.X) + t.b * a.strideX;
-  const int lane = threadIdx.x & 31;
-  for (int w = threadIdx.x >> 5; w < 16; w += 8) {
-    const int r = (w & 3) * 32 + lane, blk = w >> 2, col = tc * 128 + blk * 32;
-    if (r >= t.n || col / 32 * 16 >= a.pitch) continue;
-    float x[32];
-    uint32_t top = 0;
+  const int blk = threadIdx.x >> 6, r = (threadIdx.x & 63) * 2, col = tc * 128 + blk * 32;
+  if (r < t.n && col / 32 * 16 < a.pitch) {
+    const T *X = static_cast<const T *>(a.X) + t.b * a.strideX + (int64_t)col * a.ldx + t.r0 + r;
+    const int valid = a.cols - col;
+    const bool both = r + 1 < t.n;
+    Two<T> w[32];
+    if (both && valid >= 32 && ((uintptr_t)X % sizeof(Two<T>)) == 0 && a.ldx % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-      x[i] = col + i < a.cols ? to_float(X[(int64_t)(col + i) * a.ldx + t.r0 + r]) : 0.0f;
-      top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+      for (int i = 0; i < 32; i++) {
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t v = __ldg(reinterpret_cast<const uint32_t *>(X + i * a.ldx));
+          w[i] = *reinterpret_cast<const Two<T> *>(&v);
+        } else {
+          const uint2 v = __ldg(reinterpret_cast<const uint2 *>(X + i * a.ldx));
+          w[i] = *reinterpret_cast<const Two<T> *>(&v);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) {
+        w[i].v[0] = i < valid ? X[i * a.ldx] : T(0.0f);
+        w[i].v[1] = i < valid && both ? X[i * a.ldx + 1] : T(0.0f);
+      }
     }
-    const uint32_t e = scale_byte(top);
-    const float inv = inverse_scale(e);
-    uint32_t code[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float y[8];
+    for (int p = 0; p < 2; p++) {
+      uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = x[i * 8 + j] * inv;
-      code[i] = encode8(y);
+      for (int i = 0; i < 32; i++) top = max(top, __float_as_uint(to_float(w[i].v[p])) & 0x7fffffffu);
+      const uint32_t e = scale_byte(top);
+      const float inv = inverse_scale(e);
+      uint32_t code[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) y[k] = to_float(w[i * 8 + k].v[p]) * inv;
+        code[i] = encode8(y);
+      }
+      if (p == 0 || both) {
+        const int64_t at = ((int64_t)t.b * a.rows + t.r0 + r + p) * a.pitch + col / 2;
+        *reinterpret_cast<uint4 *>(a.codes + at) = make_uint4(code[0], code[1], code[2], code[3]);
+        sf[scale_at(r + p, blk)] = (uint8_t)e;
+      }
     }
-    const int64_t at = ((int64_t)t.b * a.rows + t.r0 + r) * a.pitch + col / 2;
-    *reinterpret_cast<uint4 *>(a.codes + at) = make_uint4(code[0], code[1], code[2], code[3]);
-    sf[(r & 31) * 16 + (r >> 5) * 4 + blk] = (uint8_t)e;
   }
   __syncthreads();
-  if (threadIdx.x < 32)
-    reinterpret_cast<uint4 *>(a.scales + ((int64_t)tile * a.tiles_c + tc) * 512)[threadIdx.x] =
-        reinterpret_cast<const uint4 *>(sf)[threadIdx.x];
+  if (threadIdx.x < 128) tile_scales(a, tile, tc)[threadIdx.x] = reinterpret_cast<const uint32_t *>(sf)[threadIdx.x];
 }
 
 // ---- the values the codes stand for ------------------------------------------
-
-// The value of a code times the scale (exact in float32: the magnitudes are
-// multiples of a half below 8).
-__device__ __forceinline__ float decode(uint32_t code, float scale) {
-  const uint32_t m = code & 7u;
-  // half steps: 0 1 2 3 4 6 8 12
-  const float v = 0.5f * (float)(m < 5 ? m : m == 5 ? 6u : m == 6 ? 8u : 12u);
-  return ((code & 8u) ? -v : v) * scale;
-}
 
 template <class T>
 __device__ __forceinline__ T from_float(float x);
@@ -224,40 +285,75 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
-// X here is the output (rows x cols, ldx).
+// Four codes' values. An element's bits moved to the low end of an fp16's exponent
+// field and the top of its mantissa are the element times 2^-14 (its exponent bias
+// is 1, fp16's 15; subnormals stay subnormal); every product below is exact.
+__device__ __forceinline__ void decode4(uint32_t code, float scale, float *y) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint32_t b = code >> (8 * i);
+    const uint32_t h = (b & 0x07u) << 9 | (b & 0x08u) << 12 | (b & 0x70u) << 21 | (b & 0x80u) << 24;
+    const float2 f = __half22float2(__hmul2(*reinterpret_cast<const __half2 *>(&h), __float2half2_rn(16384.0f)));
+    y[2 * i] = f.x * scale;
+    y[2 * i + 1] = f.y * scale;
+  }
+}
+
+// X here is the output (rows x cols, ldx). The quantiser's division of the work;
+// a thread's store is 16 bytes, a warp's 512 neighbouring ones (an fp32 line
+// takes two).
 template <class T>
 __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
+  constexpr int E = 16 / sizeof(T), PASSES = 8 / E;
   extern __shared__ int tables[];
-  __shared__ __align__(16) uint8_t sf[512];
+  __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
-  const int tile = (int)(blockIdx.x / (unsigned)a.tiles_c), tc = (int)(blockIdx.x % (unsigned)a.tiles_c);
+  const int pairs = (a.tiles_c + 1) >> 1;
+  const int tile = (int)(blockIdx.x / (unsigned)pairs), tc = (int)(blockIdx.x % (unsigned)pairs) * 2;
   const TileRows t = rows_of_tile(a, tile, tables);
   if (t.n <= 0) return;
-  if (threadIdx.x < 32)
-    reinterpret_cast<uint4 *>(sf)[threadIdx.x] =
-        reinterpret_cast<const uint4 *>(a.scales + ((int64_t)tile * a.tiles_c + tc) * 512)[threadIdx.x];
+  if (threadIdx.x < 128 || tc + 1 < a.tiles_c) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = tile_scales(a, tile, tc)[threadIdx.x];
   __syncthreads();
-  T *X = static_cast<T *>(const_cast<void *>(a.X)) + t.b * a.strideX;
-  const int c = threadIdx.x & 15, col = tc * 128 + c * 8;
-  if (col >= a.cols) return;
-  for (int r = threadIdx.x >> 4; r < t.n; r += 16) {
-    const int64_t row = t.r0 + r;
-    const uint32_t code = *reinterpret_cast<const uint32_t *>(a.codes + ((int64_t)t.b * a.rows + row) * a.pitch + col / 2);
-    const float s = scale_value(sf[(r & 31) * 16 + (r >> 5) * 4 + (c >> 2)]);
-    T *p = X + row * a.ldx + col;
-    alignas(16) T y[8];
+  const int warp = threadIdx.x >> 5, c = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = from_float<T>(decode(code >> (4 * i) & 15u, s));
-    if (col + 8 <= a.cols && ((uintptr_t)p & 15) == 0) {
+  for (int p = 0; p < PASSES; p++) {
+    const int in_tiles = p * 32 * E + c * E, col = tc * 128 + in_tiles;
+    if (col >= a.cols) return;
+    const uint8_t *src = a.codes + ((int64_t)t.b * a.rows + t.r0 + warp) * a.pitch + col / 2;
+    T *dst = static_cast<T *>(const_cast<void *>(a.X)) + t.b * a.strideX + (t.r0 + (int64_t)warp) * a.ldx + col;
+    const uint8_t *sfb = sf + scale_at(0, in_tiles >> 5);
+    const int64_t src_step = 8 * a.pitch, dst_step = 8 * a.ldx;
+    const bool wide = col + E <= a.cols && ((uintptr_t)dst & 15) == 0 && a.ldx * sizeof(T) % 16 == 0;
+    auto load = [&](const uint8_t *at) -> uint32_t {
+      if constexpr (E == 8) return __ldg(reinterpret_cast<const uint32_t *>(at));
+      else return __ldg(reinterpret_cast<const uint16_t *>(at));
+    };
+    auto store = [&](uint32_t code, T *to, int r) {
+      const float s = scale_value(sfb[(r & 31) * 16 + (r >> 5) * 4]);
+      float f[E];
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; i++)
-        reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(y)[i];
-    } else {
+      for (int i = 0; i < E / 4; i++) decode4(code >> (16 * i), s, f + 4 * i);
+      alignas(16) T y[E];
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (col + i < a.cols) p[i] = y[i];
+      for (int i = 0; i < E; i++) y[i] = from_float<T>(f[i]);
+      if (wide) {
+        *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; i++)
+          if (col + i < a.cols) to[i] = y[i];
+      }
+    };
+    int r = warp;
+    for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
+      uint32_t code[ROWS_AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step) code[u] = load(src);
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) store(code[u], dst, r + 8 * u);
     }
+    for (; r < t.n; r += 8, src += src_step, dst += dst_step) store(load(src), dst, r);
   }
 }
 
@@ -599,12 +695,12 @@ wg_status check_quant(const wg_device *d, int type, int64_t batch, int64_t rows,
   return WG_OK;
 }
 
-wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const QuantArgs), QuantArgs &a) {
+wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const QuantArgs), const QuantArgs &a, int ctas_a_row) {
   const int64_t tiles = a.offsets ? tiles_of(a.rows) + a.groups : (int64_t)a.batch * a.tiles_r;
-  if (tiles * a.tiles_c >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
+  if (tiles * ctas_a_row >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
   const size_t smem = a.offsets ? 2 * ((size_t)a.groups + 1) * sizeof(int) : 0;
   wg_launch_scope scope(d, family);
-  WG_CUDA(wg_launch_pdl(kern, dim3((unsigned)(tiles * a.tiles_c)), dim3(256), smem, d->stream, a));
+  WG_CUDA(wg_launch_pdl(kern, dim3((unsigned)(tiles * ctas_a_row)), dim3(256), smem, d->stream, a));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
 }
@@ -734,7 +830,7 @@ extern "C" wg_status wg_mx_quantize_dev(wg_device *d, int type, int trans, int64
       kern = type == WG_TYPE_F32 ? mx_quantize_t<float> : type == WG_TYPE_BF16 ? mx_quantize_t<__nv_bfloat16> : mx_quantize_t<__half>;
     else
       kern = type == WG_TYPE_F32 ? mx_quantize<float> : type == WG_TYPE_BF16 ? mx_quantize<__nv_bfloat16> : mx_quantize<__half>;
-    return launch_quant(d, "mx_quantize", kern, a);
+    return launch_quant(d, "mx_quantize", kern, a, trans ? a.tiles_c : (a.tiles_c + 1) / 2);
   });
 }
 
@@ -760,7 +856,8 @@ extern "C" wg_status wg_mx_dequantize_dev(wg_device *d, int type, int64_t batch,
   return wg_timed(d, gpu_ms, [&] {
     return launch_quant(d, "mx_dequantize",
                         type == WG_TYPE_F32 ? mx_dequantize<float>
-                        : type == WG_TYPE_BF16 ? mx_dequantize<__nv_bfloat16> : mx_dequantize<__half>, a);
+                        : type == WG_TYPE_BF16 ? mx_dequantize<__nv_bfloat16> : mx_dequantize<__half>, a,
+                        (a.tiles_c + 1) / 2);
   });
 }
 
