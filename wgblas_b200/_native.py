@@ -17,6 +17,7 @@ if not os.path.exists(LIB_PATH):
         "(wgblas_b200 has no CPU fallback)")
 
 lib = ct.CDLL(LIB_PATH)
+from . import _fast  # noqa: E402  (csrc/fastcall.c, built with the library; it calls the library loaded above)
 
 # status codes (wg_status)
 WG_OK = 0

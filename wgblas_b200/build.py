@@ -7,6 +7,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -51,7 +52,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(LIB, objs):
         subprocess.run([NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-ldl"], check=True)
     build_napi(force)
+    build_fast(force)
     return LIB
+
+
+FAST_SRC = os.path.join(CSRC, "fastcall.c")
+FAST = os.path.join(HERE, "_fast.so")
+
+
+def build_fast(force: bool = False) -> str:
+    """Builds the CPython extension _fast (csrc/fastcall.c) next to the library it calls."""
+    if force or _stale(FAST, [FAST_SRC, LIB, os.path.join(ROOT, "include", "wgblas.h")]):
+        subprocess.run(["gcc", "-std=c11", "-O2", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
+                        "-fvisibility=hidden", "-I" + os.path.join(ROOT, "include"),
+                        "-I" + sysconfig.get_paths()["include"], FAST_SRC, "-L" + HERE, "-lwgblas_b200",
+                        "-Wl,-rpath,$ORIGIN", "-o", FAST], check=True)
+    return FAST
 
 
 NAPI_SRC = os.path.join(HERE, "napi", "wgblas_napi.c")

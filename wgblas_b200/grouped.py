@@ -92,6 +92,9 @@ def gemmGrouped(device, transB, groups, m, n, k, alpha, A, lda, B, ldb, strideB,
     A is m x k, C m x n, B_g (``strideB`` elements apart; 0 shares one matrix) k x n for
     "no-transpose" or n x k for "transpose". Rows that no group holds keep their C.
     """
+    st = nat._fast.gemm_grouped(device, transB, groups, m, n, k, alpha, A, lda, B, ldb, strideB, offsets, beta, C, ldc)
+    if st is not None:  # the ordinary call, checked and made
+        return nat.check(st) or {}
     require_gpu_device(device)
     if transB not in _TRANS:
         raise Error("transB must be 'no-transpose' or 'transpose'.")
@@ -138,6 +141,9 @@ def gemmGroupedInner(device, groups, m, n, k, alpha, A, lda, B, ldb, offsets, be
     A is k x m, B k x n, C_g (``strideC`` elements apart) m x n; ``offsets`` groups the k rows.
     A group without rows gives beta * C_g.
     """
+    st = nat._fast.gemm_grouped_inner(device, groups, m, n, k, alpha, A, lda, B, ldb, offsets, beta, C, ldc, strideC)
+    if st is not None:
+        return nat.check(st) or {}
     require_gpu_device(device)
     check_scalars(alpha, beta)
     groups, m, n, k, lda, ldb, ldc, strideC = check_ints("groups, m, n, k, lda, ldb, ldc, and strideC", groups, m, n, k,

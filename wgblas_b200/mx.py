@@ -26,8 +26,8 @@ from __future__ import annotations
 import numpy as np
 
 from . import _native as nat
-from ._runtime import Error, require_gpu_device
-from .arrays import TYPE_CODES, GpuArray, disjoint, resident
+from ._runtime import Device, Error, require_gpu_device
+from .arrays import TYPE_CODES, GpuArray, _foreign_types, disjoint, resident
 from .gemm import _TRANS
 from .grouped import check_groups, check_ints, check_offsets, check_scalars, need, span, timed
 
@@ -90,6 +90,9 @@ class GpuMxMatrix:
     @staticmethod
     def wrap(device, codes, scales, rows, cols, batch=1, groups=0) -> "GpuMxMatrix":
         """A matrix in memory the caller owns."""
+        x = nat._fast.mx_wrap(device, codes, scales, rows, cols, batch, groups)
+        if x is not None:
+            return x
         return GpuMxMatrix(device, codes, scales, *GpuMxMatrix._check(device, rows, cols, batch, groups))
 
     def destroy(self) -> None:
@@ -145,6 +148,9 @@ def mxQuantize(device, trans, rows, cols, X, ldx, out, offsets=None, strideX=0):
     2^-127; elements are rounded to nearest, ties to even, beyond 6 scales to 6. A block
     with a NaN or an infinity becomes NaN.
     """
+    st = nat._fast.mx_quantize(device, trans, rows, cols, X, ldx, out, offsets, strideX)
+    if st is not None:  # the ordinary call, checked and made
+        return nat.check(st) or {}
     require_gpu_device(device)
     if trans not in _TRANS:
         raise Error("trans must be 'no-transpose' or 'transpose'.")
@@ -183,6 +189,9 @@ def mxDequantize(device, x, out, ldo, offsets=None, strideO=0):
     The matrices of a batch go ``strideO`` elements apart (by default one after the
     other). Rows that no group holds are not written.
     """
+    st = nat._fast.mx_dequantize(device, x, out, ldo, offsets, strideO)
+    if st is not None:
+        return nat.check(st) or {}
     require_gpu_device(device)
     if not isinstance(x, GpuMxMatrix):
         raise Error("x must be a GpuMxMatrix.")
@@ -244,6 +253,9 @@ def mxGemm(device, m, n, k, alpha, A, B, beta, C, ldc):
 
     C is float32, bfloat16 or float16; sums are held in 32 bits.
     """
+    st = nat._fast.mx_gemm(device, 0, m, n, k, alpha, A, B, None, beta, C, ldc)
+    if st is not None:
+        return nat.check(st) or {}
     m, n, k, ldc, pc, tc, used = _product(device, "mxGemm", m, n, k, alpha, A, B, beta, C, ldc, 0)
     if not used:
         return {}
@@ -257,6 +269,10 @@ def mxGemmGrouped(device, groups, m, n, k, alpha, A, B, offsets, beta, C, ldc):
     A is m x k with rows grouped by ``offsets`` (quantised with the same ones), B a batch
     of ``groups`` n x k matrices. Rows that no group holds keep their C.
     """
+    if groups:
+        st = nat._fast.mx_gemm(device, groups, m, n, k, alpha, A, B, offsets, beta, C, ldc)
+        if st is not None:
+            return nat.check(st) or {}
     (groups,) = check_ints("groups", groups)
     if groups < 0:
         raise Error("groups must be non-negative.")
@@ -270,6 +286,9 @@ def mxGemmGrouped(device, groups, m, n, k, alpha, A, B, offsets, beta, C, ldc):
         return {}
     return timed(device, nat.lib.wg_mx_gemm_grouped_dev, device.handle, TYPE_CODES[tc], groups, m, n, k, alpha, A._codes,
                  A._scales, B._codes, B._scales, po, beta, pc, ldc)
+
+
+nat._fast.setup(Device, GpuArray, GpuMxMatrix, _foreign_types)
 
 
 def mxDecode(codes: np.ndarray, scales: np.ndarray, rows: int, cols: int) -> np.ndarray:
