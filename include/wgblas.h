@@ -398,8 +398,8 @@ wg_status wg_dgemv_dev(wg_device *dev, int trans, int64_t m, int64_t n, double a
  * strides need only the alignment of their elements: operands whose bases are
  * 16-byte aligned and whose rows (and strideB) are whole 16-byte units are read
  * in place; others are first copied (of B, the matrices of groups with rows) to
- * a temporary of their size from the handle's stream-ordered pool. Queued on
- * the device stream; no workspace. gpu_ms as for wg_sgemm. */
+ * memory of their size from the handle's stream-ordered pool (a call captured
+ * into a graph has its own). Queued on the device stream. gpu_ms as for wg_sgemm. */
 #define WG_TYPE_F32 0
 #define WG_TYPE_BF16 1
 #define WG_TYPE_F16 2

@@ -553,7 +553,7 @@ template <int MODE>
 wg_status run(wg_device *d, Args &a, int type) {
   // Weights shared by all groups (stride 0, or one group) need no group dimension.
   a.l_group = MODE != INNER && a.groups > 1 && a.strideL != 0;
-  void *temp = nullptr;
+  wg_temp temp;
   if (a.alpha != 0.0f) {
     Realign l = {}, n = {};
     size_t bytes = 0;
@@ -578,18 +578,16 @@ wg_status run(wg_device *d, Args &a, int type) {
     }
     const size_t total = bytes + (size_t)(n.lines * n.ld_out) * 2;
     if (total) {
-      // From the handle's stream-ordered pool: captured into a graph, each graph has its own.
-      wg_status st = wg_staging_pool(d);
+      wg_status st = wg_temp_get(d, total, &temp);
       if (st != WG_OK) return st;
-      WG_CUDA(cudaMallocFromPoolAsync(&temp, total, d->staging, d->stream));
       if (l.lines) {
-        l.dst = static_cast<uint16_t *>(temp);
+        l.dst = static_cast<uint16_t *>(temp.ptr);
         a.L = l.dst;
         a.ldl = l.ld_out;
         if (a.l_group) a.strideL = l.rows * l.ld_out;
       }
       if (n.lines) {
-        n.dst = reinterpret_cast<uint16_t *>(static_cast<char *>(temp) + bytes);
+        n.dst = reinterpret_cast<uint16_t *>(static_cast<char *>(temp.ptr) + bytes);
         a.N = n.dst;
         a.ldn = n.ld_out;
       }
@@ -600,7 +598,7 @@ wg_status run(wg_device *d, Args &a, int type) {
         e = wg_launch_pdl(grouped_realign, dim3((unsigned)blocks), dim3(256), 0, d->stream, l, n);
       }
       if (e != cudaSuccess) {
-        cudaFreeAsync(temp, d->stream);
+        wg_temp_done(d, &temp);
         return wg_fail(WG_ERR_CUDA, "grouped_realign failed: %s", cudaGetErrorString(e));
       }
     }
@@ -614,11 +612,8 @@ wg_status run(wg_device *d, Args &a, int type) {
   if (pair) st = launch<MODE, Shape<2, 256>>(d, a, type);
   else if (MODE != INNER && avg <= 32) st = launch<MODE, Shape<1, 32>>(d, a, type);
   else st = launch<MODE, Shape<1, 128>>(d, a, type);
-  if (temp) {
-    const cudaError_t e = cudaFreeAsync(temp, d->stream);
-    if (st == WG_OK) WG_CUDA(e);
-  }
-  return st;
+  const wg_status done = wg_temp_done(d, &temp);
+  return st == WG_OK ? done : st;
 }
 
 wg_status check_common(const wg_device *d, int type, int ctype, int64_t groups, int64_t m, int64_t n, int64_t k) {

@@ -95,6 +95,9 @@ struct wg_device {
   size_t flow_flags_n;
   uint32_t flow_epoch;
   cudaStream_t h2d, d2h;  // copy streams of the host-array path (created on first use)
+  void *temp;         // memory wg_temp_get keeps, last used on temp_stream
+  size_t temp_bytes;
+  cudaStream_t temp_stream;
   cudaMemPool_t staging;  // device copies of host-array operands; keeps its memory between calls
   // panelled 3xTF32 products: the stream their operand splits run on, and events
   // (entry, op(A) split ready, a panel's op(B) split ready, split buffer 0/1 free)
@@ -247,6 +250,18 @@ void wg_tc_product_join(wg_tc_product *p);
 
 // Returns at least `bytes` of device scratch owned by the handle (stream-ordered reuse).
 wg_status wg_workspace(wg_device *dev, size_t bytes, void **ptr);
+// `bytes` of device memory for the work queued next on d->stream; give it back
+// with wg_temp_done after queueing. While the stream is captured it is an
+// allocation of its own in the graph, so graphs share nothing. On the handle's
+// own stream and the legacy stream, which are never destroyed, it is kept for
+// the next call (in stream order; allocating and freeing between kernels costs
+// about 10 us a call), on other streams it comes from and returns to the pool.
+struct wg_temp {
+  void *ptr = nullptr;
+  bool pooled = false;
+};
+wg_status wg_temp_get(wg_device *dev, size_t bytes, wg_temp *out);
+wg_status wg_temp_done(wg_device *dev, wg_temp *t);
 // The device's stream-ordered memory pool (created on first use, destroyed
 // with the handle). It keeps the memory it has mapped when allocations are
 // freed, so repeated temporaries of the same sizes cost no mapping.

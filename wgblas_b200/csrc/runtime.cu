@@ -115,6 +115,10 @@ extern "C" wg_status wg_device_close(wg_device *d) {
   wg_device_guard guard(d->ordinal);
   cudaStreamSynchronize(d->stream);
   if (d->ws) cudaFree(d->ws);
+  if (d->temp) {
+    cudaFreeAsync(d->temp, d->temp_stream);
+    cudaStreamSynchronize(d->temp_stream);  // before its pool goes
+  }
   if (d->flow_flags) cudaFree(d->flow_flags);
   if (d->dwords) cudaFree(d->dwords);
   cudaEventDestroy(d->ev_start);
@@ -367,6 +371,40 @@ wg_status wg_staging_pool(wg_device *d) {
     return wg_fail(WG_ERR_CUDA, "cudaMemPoolSetAttribute failed: %s", cudaGetErrorString(e));
   }
   d->staging = pool;
+  return WG_OK;
+}
+
+wg_status wg_temp_get(wg_device *d, size_t bytes, wg_temp *out) {
+  wg_status st = wg_staging_pool(d);
+  if (st != WG_OK) return st;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  const bool kept = d->stream == d->own_stream || d->stream == cudaStreamLegacy;
+  // (the legacy stream cannot be captured, and must not be asked while another stream is)
+  if (d->stream != cudaStreamLegacy) WG_CUDA(cudaStreamIsCapturing(d->stream, &cap));
+  if (!kept || cap != cudaStreamCaptureStatusNone) {
+    WG_CUDA(cudaMallocFromPoolAsync(&out->ptr, bytes, d->staging, d->stream));
+    out->pooled = true;
+    return WG_OK;
+  }
+  if (d->temp && (d->temp_stream != d->stream || d->temp_bytes < bytes)) {
+    void *old = d->temp;
+    d->temp = nullptr;
+    d->temp_bytes = 0;
+    WG_CUDA(cudaFreeAsync(old, d->temp_stream));
+  }
+  if (!d->temp) {
+    const size_t want = (bytes + ((size_t)1 << 21) - 1) & ~(((size_t)1 << 21) - 1);
+    WG_CUDA(cudaMallocFromPoolAsync(&d->temp, want, d->staging, d->stream));
+    d->temp_bytes = want;
+    d->temp_stream = d->stream;
+  }
+  out->ptr = d->temp;
+  return WG_OK;
+}
+
+wg_status wg_temp_done(wg_device *d, wg_temp *t) {
+  if (t->ptr && t->pooled) WG_CUDA(cudaFreeAsync(t->ptr, d->stream));
+  t->ptr = nullptr;
   return WG_OK;
 }
 
