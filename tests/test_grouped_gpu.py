@@ -174,6 +174,16 @@ def test_rows_pairs_long(wg, device):
     run_rows(wg, device, N, [700, 300], 9600, 2056, "float16")
 
 
+@pytest.mark.parametrize("trans", [T, N])
+@pytest.mark.parametrize("sizes,n,k", [([3], 200, 2048), ([1], 128, 8200), ([32, 0, 1, 33, 7], 520, 1030), ([64, 50], 136, 4096),
+                                       ([40, 0, 70], 264, 3000), ([17] * 12, 264, 600), ([5], 1024, 65), ([70], 136, 100)])
+@pytest.mark.parametrize("ctype", ["bfloat16", "float32"])
+def test_rows_split_contraction(wg, device, trans, sizes, n, k, ctype):
+    """Few tiles and a long contraction: several CTAs share a tile."""
+    run_rows(wg, device, trans, sizes, n, k, ctype=ctype, first=1, after=2)
+    run_rows(wg, device, trans, sizes, n, k, ctype=ctype, alpha=0.5, beta=-1.0)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_odd_many_tiles_and_long(wg, device, dtype):
     run_rows(wg, device, T, [700, 300], 1001, 2049, dtype, "float32")
@@ -243,6 +253,12 @@ def test_inner_pairs(wg, device, m, n, ctype):
     sizes = [150, 0, 1, 17, 63, 64, 65, 512, 513, 530, 128, 1100, 16, 31, 700, 5]
     run_inner(wg, device, sizes, m, n, ctype=ctype, first=2, after=3, poison=np.nan)
     run_inner(wg, device, sizes, m, n, ctype=ctype, alpha=0.5, beta=1.0, pad=(8, 16, 3, 5))
+
+
+def test_inner_split_contraction(wg, device):
+    run_inner(wg, device, [3000], 136, 264, first=1, after=2, poison=np.nan)
+    run_inner(wg, device, [1500, 0, 40, 777], 130, 200, ctype="bfloat16", alpha=0.5, beta=1.0)
+    run_inner(wg, device, [129], 64, 136)
 
 
 def test_inner_long(wg, device):

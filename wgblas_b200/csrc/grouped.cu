@@ -46,21 +46,25 @@ constexpr size_t SMEM_LIMIT = 227 * 1024;
 //   INNER   both MN-major (rows of A and of B are the contraction)
 enum { ROWS_T = 0, ROWS_N = 1, INNER = 2 };
 
-template <int CG_, int BN_>
+// CG CTAs (a pair or one) share a tile's lanes, P CTAs its contraction.
+template <int CG_, int BN_, int P_ = 1>
 struct Shape {
-  static constexpr int CG = CG_, BN = BN_;
+  static constexpr int CG = CG_, BN = BN_, P = P_, CLUSTER = CG * P;
+  static_assert(CG == 1 || P == 1, "a pair shares lanes or contraction, not both");
   static constexpr int TL = CG * BL;            // lanes of a tile
   static constexpr int CPT = BN / 2;            // accumulator columns of an epilogue thread
   static constexpr int L_BYTES = BL * 128;
   static constexpr int N_BYTES = BN / CG * 128;  // each CTA of a pair holds half of the columns' lines
   static constexpr int STAGE = L_BYTES + N_BYTES;
+  static constexpr int PARTS = (P - 1) * BN * BL * 4;
   static constexpr int MAX_STAGES = 10;
-  // Ring depth: what shared memory holds beside the groups' tables.
-  static constexpr int STAGES = (int)((SMEM_LIMIT - 12 * 1024) / STAGE) < MAX_STAGES
-                                    ? (int)((SMEM_LIMIT - 12 * 1024) / STAGE)
-                                    : MAX_STAGES;
-  static constexpr int BARS = 4 * STAGES + 4;
-  static constexpr size_t tables = (size_t)STAGES * STAGE + (BARS * 8 + 8 + 15) / 16 * 16;
+  // Ring depth: what shared memory holds beside the groups' tables and the parts.
+  static constexpr int FIT = (int)((SMEM_LIMIT - 12 * 1024 - PARTS) / STAGE);
+  static constexpr int STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
+  static constexpr int BARS = 4 * STAGES + 6;
+  static constexpr size_t parts = (size_t)STAGES * STAGE;
+  static constexpr size_t bars = parts + PARTS;
+  static constexpr size_t tables = bars + (BARS * 8 + 8 + 15) / 16 * 16;
   static constexpr size_t smem(int groups) { return 1024 + tables + 2 * ((size_t)groups + 1) * sizeof(int); }
   static constexpr int NMMA_STEP = CG * 16;
 };
@@ -73,10 +77,8 @@ struct Args {
   int k;         // rows form: contraction length
   int tiles_l, tiles_n;
   const int *offsets;
-  float alpha, beta;
-  void *C;
-  int64_t ldc, strideC;
-  int ctype;
+  wgg::Out out;
+  int64_t strideC;
   uint32_t ab_format;  // idesc a/b format: 0 fp16, 1 bf16
   int l_group;         // 1: the L side's map has a group dimension (0: all groups share one matrix)
   // the operands
@@ -127,10 +129,11 @@ struct Tile {
   int r0;     // rows form: the tile's first row; inner form: the group's first row
   int kt;     // k-blocks
   int klen;   // contraction length
+  int k_lo, k_hi;  // this CTA's k-blocks
 };
 
 template <int MODE, class S>
-__device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *start, const int *tile0) {
+__device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *start, const int *tile0, uint32_t rank) {
   Tile x;
   if (MODE == INNER) {
     const int per = a.tiles_l * a.tiles_n;
@@ -160,7 +163,9 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
     x.nv = min(each, rows - first);
     x.klen = a.k;
   }
-  x.kt = a.alpha == 0.0f ? 0 : (x.klen + BK - 1) / BK;
+  x.kt = a.out.alpha == 0.0f ? 0 : (x.klen + BK - 1) / BK;
+  x.k_lo = S::P > 1 ? (int)((int64_t)x.kt * rank / S::P) : 0;
+  x.k_hi = S::P > 1 ? (int)((int64_t)x.kt * (rank + 1) / S::P) : x.kt;
   return x;
 }
 
@@ -188,19 +193,20 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = wgtc::smem_addr(smem_raw);
   uint8_t *smem = smem_raw + ((1024 - (base & 1023)) & 1023);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + (size_t)STAGES * S::STAGE);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::bars);
   uint64_t *empty = full + STAGES;
   uint64_t *tail = empty + STAGES;       // inner form: this CTA's ragged last block has landed
   uint64_t *tail_peer = tail + STAGES;   // ... and the other CTA of a pair has zeroed what is past its end
   uint64_t *acc_full = tail_peer + STAGES;  // [2]
   uint64_t *acc_empty = acc_full + 2;       // [2]
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  wgg::Parts parts = {reinterpret_cast<float *>(smem + S::parts), acc_empty + 2, acc_empty + 3, 0};
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 4);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *start = reinterpret_cast<int *>(smem + S::tables);
   int *tile0 = start + a.groups + 1;
 
   const int warp = wgg::warp_index(), lane = threadIdx.x & 31;
-  const uint32_t rank = wgg::pair_rank<CG>();
+  const uint32_t rank = S::CLUSTER > 1 ? wgtc::cluster_ctarank() : 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
       wgtc::mbar_init(&full[s], 2);
@@ -212,6 +218,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       wgtc::mbar_init(&acc_full[b], 1);
       wgtc::mbar_init(&acc_empty[b], CG * EPI_WARPS);
     }
+    wgtc::mbar_init(parts.full, EPI_WARPS * (S::P > 1 ? S::P - 1 : 1));
+    wgtc::mbar_init(parts.empty, EPI_WARPS);
     *abort_flag = 0;
     wgtc::fence_barrier_init();
   }
@@ -222,12 +230,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   wg_pdl_trigger();
   wgg::plan_groups(a.offsets, a.groups, a.rows, S::BN, start, MODE == INNER ? nullptr : tile0, nullptr, a.dwords);
   wgtc::tc_fence_before();
-  wgg::pair_sync<CG>();
+  wgg::cluster_sync<S::CLUSTER>();
   wgtc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int64_t tiles = MODE == INNER ? (int64_t)a.groups * a.tiles_l * a.tiles_n
                                       : (int64_t)tile0[a.groups] * a.tiles_l;
-  const int64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
+  const int64_t t_first = blockIdx.x / S::CLUSTER, t_step = gridDim.x / S::CLUSTER;
+  const uint32_t half = CG == 2 ? rank : 0;  // which lanes and columns of a pair's tile
 
   // A wait that gives up records it and tells the other roles to stop at their
   // next failed wait (each is bounded on its own).
@@ -243,14 +252,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     const bool l_side = warp == 0;
     const uint32_t lead = wgg::leader_addr<CG>(full);
     for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-      const Tile x = tile_at<MODE, S>(a, t, start, tile0);
-      const int half = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
+      const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
+      const int cols = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
       // The first box's outer coordinate, and how many boxes.
-      const int c0 = l_side ? x.l0 + (int)rank * BL : (N_MN ? x.n0 : x.r0) + (int)rank * half;
-      const int boxes = l_side ? 2 : (half + NBOX - 1) / NBOX;
+      const int c0 = l_side ? x.l0 + (int)half * BL : (N_MN ? x.n0 : x.r0) + (int)half * cols;
+      const int boxes = l_side ? 2 : (cols + NBOX - 1) / NBOX;
       const uint32_t bytes = (uint32_t)(l_side ? S::L_BYTES : boxes * NBOX * 128);
       const int lg = x.g * a.l_group;
-      for (int kb = 0; kb < x.kt; kb++, ring.next()) {
+      for (int kb = x.k_lo; kb < x.k_hi; kb++, ring.next()) {
         const int s = ring.s;
         ok = wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET);
         ok = __all_sync(0xffffffffu, ok);
@@ -265,7 +274,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
             for (int b = 0; b < boxes; b++)
               wgtc::tma_load_2d(dst + b * CHUNK, l_side ? &map_l : &map_n, &tail[s], c0 + b * 64, k0);
           } else {
-            if (rank == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
+            if (half == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
             if (l_side) {
               if (MODE == ROWS_T) {
                 wgg::load_3d<CG>(dst, &map_l, &full[s], at, k0, c0, lg);
@@ -297,16 +306,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     int s = 0;
     uint32_t phase = 0;  // parity of tail[s], tail_peer[s] at bit s
     for (int64_t t = t_first; t < tiles; t += t_step) {
-      const Tile x = tile_at<MODE, S>(a, t, start, tile0);
-      if (x.kt == 0) continue;
-      s = (s + x.kt - 1) % STAGES;  // the tile's last block
-      const int left = x.klen - (x.kt - 1) * BK;
-      if (left & 15) {
+      const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
+      if (x.k_hi == x.k_lo) continue;
+      s = (s + x.k_hi - x.k_lo - 1) % STAGES;  // this CTA's last block
+      const int left = x.klen - (x.k_hi - 1) * BK;  // (64 or more in front of another CTA's)
+      if (left < BK && (left & 15)) {
         const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
         bool ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&tail[s], phase >> s & 1u, WAIT_BUDGET));
         if (ok) {
           zero_tail(smem + (size_t)s * S::STAGE, left, 2 + (nmma / CG + 63) / 64, lane);
-          if (CG == 2 && rank == 1) {
+          if (CG == 2 && half == 1) {
             if (lane == 0) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(&tail_peer[s]), 0));
           } else {
             if (CG == 2)
@@ -324,7 +333,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       if (++s == STAGES) s = 0;
     }
   } else if (warp == 1) {
-    if (rank == 0) {
+    if (half == 0) {
       // ---- MMA issuer ----
       wgg::Ring<STAGES> ring;
       int used = 0;
@@ -335,11 +344,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       const uint64_t desc_n0 = N_MN ? smem_desc_mn(smem0 + S::L_BYTES) : wgtc::smem_desc_kmajor(smem0 + S::L_BYTES, 128);
       bool ok = true;
       for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-        const Tile x = tile_at<MODE, S>(a, t, start, tile0);
+        const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
         const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
         const uint32_t idesc = idesc_f16(a.ab_format, S::TL, nmma, L_MN, N_MN);
-        for (int kb0 = 0; kb0 < x.kt && ok; kb0 += segment, used++) {
-          const int b = used & 1, kb1 = min(x.kt, kb0 + segment);
+        for (int kb0 = x.k_lo; kb0 < x.k_hi && ok; kb0 += segment, used++) {
+          const int b = used & 1, kb1 = min(x.k_hi, kb0 + segment);
           const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
           ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET));
           wgtc::tc_fence_after();
@@ -387,28 +396,37 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       used++;
     };
     for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-      const Tile x = tile_at<MODE, S>(a, t, start, tile0);
+      const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
       const int valid = x.nv - h * S::CPT;  // columns this warp has (may be none)
-      const int l = x.l0 + (int)rank * BL + q * 32 + lane;
+      const int l = x.l0 + (int)half * BL + q * 32 + lane;
       const int64_t row = (MODE == INNER ? x.n0 : x.r0) + h * S::CPT;
-      const int64_t at = (MODE == INNER ? (int64_t)x.g * a.strideC : 0) + row * a.ldc + l;
+      const int64_t at = (MODE == INNER ? (int64_t)x.g * a.strideC : 0) + row * a.out.ldc + l;
       const uint32_t col = tmem + (uint32_t)(h * S::CPT) + ((uint32_t)(q * 32) << 16);
-      if constexpr (SUMS) {
+      if constexpr (SUMS || S::P > 1) {
         float sum[S::CPT];
 #pragma unroll
         for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
-        for (int kb0 = 0; kb0 < x.kt; kb0 += SEG) {
+        for (int kb0 = x.k_lo; kb0 < x.k_hi; kb0 += SUMS ? SEG : 1 << 30) {
           const int b = used & 1;
           if (!(ok = wait_acc(b))) break;
-          wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == 0, sum);
+          wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == x.k_lo, sum);
           free_acc(b);
         }
-        if (ok && l < a.nl) wgg::store_sums<S::CPT>(static_cast<float *>(a.C) + at, a.ldc, valid, a.alpha, a.beta, sum);
+        if (!ok) break;
+        bool mine = true;
+        if constexpr (S::P > 1) {
+          if (x.kt) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, sum, &ok);
+          else mine = rank == 0;
+          if (!ok) {
+            if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
+            break;
+          }
+        }
+        if (mine) wgg::store_sums<S::CPT, SUMS && S::P == 1>(a.out, at, l < a.nl, valid, sum);
       } else {
         const int b = used & 1;
         if (x.kt && !(ok = wait_acc(b))) break;
-        wgg::store_acc<S::CPT>(col + (uint32_t)(b * S::BN), x.kt != 0, a.C, a.ctype, at, a.ldc, valid, l < a.nl, a.alpha,
-                               a.beta);
+        wgg::store_acc<S::CPT>(col + (uint32_t)(b * S::BN), x.kt != 0, a.out, at, l < a.nl, valid);
         if (x.kt) free_acc(b);
       }
     }
@@ -416,7 +434,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
 
   wgtc::tc_fence_before();
   __syncwarp();
-  wgg::pair_sync<CG>();
+  wgg::cluster_sync<S::CLUSTER>();
   if (warp == 1) {
     wgtc::tc_fence_after();
     wgg::pair_tmem_dealloc<CG>(tmem, 2 * S::BN);
@@ -527,10 +545,10 @@ wg_status launch_as(wg_device *d, Args &a, const CUtensorMap &ml, const CUtensor
   a.tiles_n = MODE == INNER ? (a.nn + S::BN - 1) / S::BN : 0;
   const int64_t most = (int64_t)a.tiles_l * (MODE == INNER ? (int64_t)a.groups * a.tiles_n
                                                            : (int64_t)a.rows / S::BN + a.groups);
-  const unsigned grid = S::CG * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CG));
+  const unsigned grid = S::CLUSTER * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CLUSTER));
   wg_launch_scope scope(d, MODE == INNER ? "gemm_grouped_inner" : "gemm_grouped");
   WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, SUMS>, SMEM_LIMIT));
-  WG_CUDA((wgg::launch<S::CG>(grouped_kernel<MODE, S, SUMS>, grid, MODE == INNER ? 384 : 352, S::smem(a.groups),
+  WG_CUDA((wgg::launch<S::CLUSTER>(grouped_kernel<MODE, S, SUMS>, grid, MODE == INNER ? 384 : 352, S::smem(a.groups),
                               d->stream, ml, mn, a)));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
@@ -542,11 +560,49 @@ wg_status launch(wg_device *d, Args &a, int type) {
   memset(&ml, 0, sizeof ml);
   memset(&mn, 0, sizeof mn);
   // (no product, no operands)
-  if (a.alpha != 0.0f && !make_maps<MODE, S>(a, type, &ml, &mn))
+  if (a.out.alpha != 0.0f && !make_maps<MODE, S>(a, type, &ml, &mn))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
   // One accumulator holds at most SEG k-blocks' sums of an fp32 result.
-  const bool sums = a.ctype == WG_TYPE_F32 && (MODE == INNER ? a.rows : a.k) > SEG * BK;
-  return sums ? launch_as<MODE, S, true>(d, a, ml, mn) : launch_as<MODE, S, false>(d, a, ml, mn);
+  // (a split contraction's sums are always drained, and few blocks long)
+  const bool sums = S::P > 1 || (a.out.type == WG_TYPE_F32 && (MODE == INNER ? a.rows : a.k) > SEG * BK);
+  if constexpr (S::P > 1) return launch_as<MODE, S, true>(d, a, ml, mn);
+  else return sums ? launch_as<MODE, S, true>(d, a, ml, mn) : launch_as<MODE, S, false>(d, a, ml, mn);
+}
+
+// The form with the least modelled time. A form's tiles run in rounds over the
+// SMs; a round takes its k-blocks times the larger of the tensor core's time and
+// the time an SM needs to receive the block (65 bytes a clock from L2), or the
+// clocks that issuing it takes; joining a split contraction adds a fixed time.
+// Groups are taken to be evenly filled: the host does not know their sizes.
+enum Form { PAIR_256, ONE_128, ONE_64, ONE_32, SPLIT_64, SPLIT_32_2, SPLIT_32_4, FORMS };
+template <int MODE>
+Form choose(const wg_device *d, const Args &a) {
+  static const struct { int cg, bn, p; } forms[FORMS] = {{2, 256, 1}, {1, 128, 1}, {1, 64, 1}, {1, 32, 1},
+                                                         {1, 64, 2}, {1, 32, 2}, {1, 32, 4}};
+  const int64_t groups = MODE == INNER ? a.groups : std::max<int64_t>(1, std::min(a.groups, a.rows));
+  const int64_t cols = MODE == INNER ? a.nn : (a.rows + groups - 1) / groups;  // of one group
+  const int64_t klen = MODE == INNER ? (a.rows + groups - 1) / groups : a.k;
+  const int64_t kt = std::max<int64_t>(1, (klen + BK - 1) / BK);
+  Form best = ONE_128;
+  double least = 1e300;
+  for (int i = 0; i < FORMS; i++) {
+    const auto f = forms[i];
+    if (MODE == INNER && f.bn < 64) continue;
+    const int64_t nt = (cols + f.bn - 1) / f.bn, nv = MODE == INNER ? std::min<int64_t>(cols, f.bn) : (cols + nt - 1) / nt;
+    const int64_t tl = (a.nl + f.cg * BL - 1) / (f.cg * BL), slots = f.p == 4 ? d->sm_count * 7 / 32 : d->sm_count / (f.cg * f.p);
+    const int64_t rounds = (tl * groups * nt + slots - 1) / slots;
+    const int64_t box = std::min<int64_t>(f.bn, 64), lines = (nv / f.cg + box - 1) / box * box;
+    const double mma = nv * 2.0;  // 4 MMAs of 16: 2 clocks a column (128 or 256 lanes)
+    const double block = std::max({mma, (BL + lines) * 128 / 65.0, 230.0});
+    // A tile's results: the last round's are stored in the open (20 bytes a clock).
+    const double tail = (double)BL * nv * (a.out.type == WG_TYPE_F32 ? 4 : 2) / 20 + (f.p > 1 ? 2500 : 0);
+    const double t = rounds * (double)((kt + f.p - 1) / f.p) * block + tail;
+    if (t < least) {
+      least = t;
+      best = (Form)i;
+    }
+  }
+  return best;
 }
 
 template <int MODE>
@@ -554,7 +610,7 @@ wg_status run(wg_device *d, Args &a, int type) {
   // Weights shared by all groups (stride 0, or one group) need no group dimension.
   a.l_group = MODE != INNER && a.groups > 1 && a.strideL != 0;
   wg_temp temp;
-  if (a.alpha != 0.0f) {
+  if (a.out.alpha != 0.0f) {
     Realign l = {}, n = {};
     size_t bytes = 0;
     if (!mappable(a.L, a.ldl, a.l_group ? a.strideL : 0)) {
@@ -603,15 +659,22 @@ wg_status run(wg_device *d, Args &a, int type) {
       }
     }
   }
-  const int64_t avg = (a.rows + a.groups - 1) / a.groups;
-  // Tiles the pair form would have (rows form: at least).
-  const int64_t pairs = (int64_t)((a.nl + 255) / 256) *
-                        (MODE == INNER ? (int64_t)a.groups * ((a.nn + 255) / 256) : std::max<int64_t>(a.groups, a.rows / 256));
-  const bool pair = (MODE == INNER ? a.nn > 128 : avg > 128) && 2 * pairs >= d->sm_count;
   wg_status st;
-  if (pair) st = launch<MODE, Shape<2, 256>>(d, a, type);
-  else if (MODE != INNER && avg <= 32) st = launch<MODE, Shape<1, 32>>(d, a, type);
-  else st = launch<MODE, Shape<1, 128>>(d, a, type);
+  const Form form = choose<MODE>(d, a);
+  switch (form) {
+    case PAIR_256: st = launch<MODE, Shape<2, 256>>(d, a, type); break;
+    case ONE_128: st = launch<MODE, Shape<1, 128>>(d, a, type); break;
+    case ONE_64: st = launch<MODE, Shape<1, 64>>(d, a, type); break;
+    case SPLIT_64: st = launch<MODE, Shape<1, 64, 2>>(d, a, type); break;
+    default:
+      if constexpr (MODE == INNER) {
+        st = WG_ERR_INVALID_ARGUMENT;  // (not chosen: 64 columns are the least an MN-major side has)
+      } else {
+        st = form == ONE_32 ? launch<MODE, Shape<1, 32>>(d, a, type)
+             : form == SPLIT_32_2 ? launch<MODE, Shape<1, 32, 2>>(d, a, type)
+                               : launch<MODE, Shape<1, 32, 4>>(d, a, type);
+      }
+  }
   const wg_status done = wg_temp_done(d, &temp);
   return st == WG_OK ? done : st;
 }
@@ -676,11 +739,7 @@ extern "C" wg_status wg_gemm_grouped_dev(wg_device *d, int type, int ctype, int 
   a.nl = (int)n;
   a.k = (int)k;
   a.offsets = offsets;
-  a.alpha = k > 0 ? alpha : 0.0f;
-  a.beta = beta;
-  a.C = C;
-  a.ldc = ldc;
-  a.ctype = ctype;
+  a.out = {C, ldc, k > 0 ? alpha : 0.0f, beta, ctype};
   a.ab_format = type == WG_TYPE_BF16 ? 1u : 0u;
   a.L = static_cast<const uint16_t *>(B);
   a.ldl = ldb;
@@ -718,12 +777,8 @@ extern "C" wg_status wg_gemm_grouped_inner_dev(wg_device *d, int type, int ctype
   a.nl = (int)n;
   a.nn = (int)m;
   a.offsets = offsets;
-  a.alpha = k > 0 ? alpha : 0.0f;
-  a.beta = beta;
-  a.C = C;
-  a.ldc = ldc;
   a.strideC = groups > 1 ? strideC : 0;
-  a.ctype = ctype;
+  a.out = {C, ldc, k > 0 ? alpha : 0.0f, beta, ctype};
   a.ab_format = type == WG_TYPE_BF16 ? 1u : 0u;
   a.L = static_cast<const uint16_t *>(B);
   a.ldl = ldb;

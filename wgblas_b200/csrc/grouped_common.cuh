@@ -121,21 +121,45 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
 
 // ---- epilogue ----------------------------------------------------------------
 
-// Stores W sums of one lane: row r0 + j of C (ldc apart), for j < valid. alpha,
-// beta as in BLAS (C is read only when beta != 0), in 32 bits, rounded once to
-// C's type. `at` points at the lane's element of the first row.
-template <class T, int W, class Round>
-__device__ __forceinline__ void store_typed(T *at, int64_t ldc, int valid, float alpha, float beta, const float *acc,
-                                            Round round) {
-  // (pointers step by ldc: W addresses kept apart would not fit the registers)
+// Where and how results are stored: alpha, beta as in BLAS (C is read only when
+// beta != 0), in 32 bits, rounded once to C's type. Lane i of a warp holds column
+// l0 + i of W rows of C (ldc apart), of which the first `valid` exist. What bounds
+// the stores is the rate at which an SM writes to L2, about 28 bytes a clock
+// (measured with stores alone; this code reaches about 20): exchanging values
+// between lanes to store 16-bit results as pairs, half as many stores, gained
+// nothing.
+struct Out {
+  void *C;
+  int64_t ldc;
+  float alpha, beta;
+  int type;
+};
+
+template <class T>
+__device__ __forceinline__ T round_to(float x);
+template <>
+__device__ __forceinline__ float round_to<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half round_to<__half>(float x) { return __float2half_rn(x); }
+
+// One column a lane. `at`: the element of row 0 in this lane's column. (The
+// pointers step by ldc: W addresses kept apart would not fit the registers.)
+template <class T, int W>
+__device__ __forceinline__ void store_single(const Out &o, int64_t at, bool in, int valid, const float *acc) {
+  if (!in) return;
+  T *p = static_cast<T *>(o.C) + at;
+  const int64_t ldc = o.ldc;
+  const float alpha = o.alpha, beta = o.beta;
   if (beta == 0.0f) {
     if (valid >= W) {
 #pragma unroll
-      for (int j = 0; j < W; j++, at += ldc) *at = round(alpha * acc[j]);
+      for (int j = 0; j < W; j++, p += ldc) *p = round_to<T>(alpha * acc[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < W; j++, at += ldc)
-        if (j < valid) *at = round(alpha * acc[j]);
+      for (int j = 0; j < W; j++, p += ldc)
+        if (j < valid) *p = round_to<T>(alpha * acc[j]);
     }
     return;
   }
@@ -143,27 +167,21 @@ __device__ __forceinline__ void store_typed(T *at, int64_t ldc, int valid, float
   // round trip for them.
 #pragma unroll
   for (int c = 0; c < W; c += 8) {
-    T old[8], *p = at;
+    T old[8], *r = p;
+#pragma unroll
+    for (int j = 0; j < 8; j++, r += ldc)
+      if (c + j < valid) old[j] = *r;
 #pragma unroll
     for (int j = 0; j < 8; j++, p += ldc)
-      if (c + j < valid) old[j] = *p;
-#pragma unroll
-    for (int j = 0; j < 8; j++, at += ldc)
-      if (c + j < valid) *at = round(fmaf(beta, (float)old[j], alpha * acc[c + j]));
+      if (c + j < valid) *p = round_to<T>(fmaf(beta, (float)old[j], alpha * acc[c + j]));
   }
 }
 
 template <int W>
-__device__ __forceinline__ void store_cols(void *C, int type, int64_t at, int64_t ldc, int valid, float alpha,
-                                           float beta, const float *acc) {
-  if (type == WG_TYPE_BF16)
-    store_typed<__nv_bfloat16, W>(static_cast<__nv_bfloat16 *>(C) + at, ldc, valid, alpha, beta, acc,
-                                  [](float x) { return __float2bfloat16_rn(x); });
-  else if (type == WG_TYPE_F16)
-    store_typed<__half, W>(static_cast<__half *>(C) + at, ldc, valid, alpha, beta, acc,
-                           [](float x) { return __float2half_rn(x); });
-  else
-    store_typed<float, W>(static_cast<float *>(C) + at, ldc, valid, alpha, beta, acc, [](float x) { return x; });
+__device__ __forceinline__ void store_cols(const Out &o, int64_t at, bool in, int valid, const float *acc) {
+  if (o.type == WG_TYPE_F32) store_single<float, W>(o, at, in, valid, acc);
+  else if (o.type == WG_TYPE_BF16) store_single<__nv_bfloat16, W>(o, at, in, valid, acc);
+  else store_single<__half, W>(o, at, in, valid, acc);
 }
 
 // Eight epilogue warps: warp w of them reads lane quarter w % 4 and its half
@@ -186,26 +204,20 @@ __device__ __forceinline__ void drain(uint32_t taddr, int valid, bool first, flo
   }
 }
 
-template <int CPT>
-__device__ __forceinline__ void store_sums(float *at, int64_t ldc, int valid, float alpha, float beta,
-                                           const float (&sum)[CPT]) {
-#pragma unroll
-  for (int c = 0; c < CPT; c += 16, at += 16 * ldc)
-    if (c < valid) store_typed<float, 16>(at, ldc, valid - c, alpha, beta, sum + c, [](float x) { return x; });
-}
-
-template <int CPT>
-__device__ __forceinline__ void store_all(void *C, int type, int64_t at, int64_t ldc, int valid, float alpha,
-                                          float beta, const float (&sum)[CPT]) {
+// Stores drained sums; FP32: C is float32 whatever o.type says.
+template <int CPT, bool FP32>
+__device__ __forceinline__ void store_sums(const Out &o, int64_t at, bool in, int valid, const float (&sum)[CPT]) {
 #pragma unroll
   for (int c = 0; c < CPT; c += 16)
-    if (c < valid) store_cols<16>(C, type, at + (int64_t)c * ldc, ldc, valid - c, alpha, beta, sum + c);
+    if (c < valid) {
+      if (FP32) store_single<float, 16>(o, at + (int64_t)c * o.ldc, in, valid - c, sum + c);
+      else store_cols<16>(o, at + (int64_t)c * o.ldc, in, valid - c, sum + c);
+    }
 }
 
 // Stores CPT accumulator columns straight from TMEM (`from` false: zeros instead).
 template <int CPT>
-__device__ __forceinline__ void store_acc(uint32_t taddr, bool from, void *C, int type, int64_t at, int64_t ldc,
-                                          int valid, bool in, float alpha, float beta) {
+__device__ __forceinline__ void store_acc(uint32_t taddr, bool from, const Out &o, int64_t at, bool in, int valid) {
   constexpr int W = CPT < 32 ? CPT : 32;
   static_assert(W == 16 || W == 32, "");
 #pragma unroll 1
@@ -219,8 +231,59 @@ __device__ __forceinline__ void store_acc(uint32_t taddr, bool from, void *C, in
     }
 #pragma unroll
     for (int j = 0; j < W; j++) f[j] = from ? __uint_as_float(r[j]) : 0.0f;
-    if (in) store_cols<W>(C, type, at + (int64_t)c * ldc, ldc, valid - c, alpha, beta, f);
+    store_cols<W>(o, at + (int64_t)c * o.ldc, in, valid - c, f);
   }
+}
+
+// ---- contraction split over a cluster --------------------------------------------
+//
+// P CTAs of a cluster share a tile, each with its part of the k-blocks; CTA 0
+// adds the others' sums to its own, in the order of their parts, and stores.
+// Their epilogue warps write them into its shared memory, [part][column][lane],
+// when its warps have read the last tile's.
+
+struct Parts {
+  float *buf;        // CTA 0: (P - 1) x BN x 128 sums
+  uint64_t *full;    // CTA 0: the others' sums have arrived (8 warps x (P - 1) arrivals)
+  uint64_t *empty;   // others: CTA 0 has read them (8 arrivals)
+  uint32_t turn;     // exchanges so far
+};
+
+// Joins sum[] over the cluster; true on CTA 0, which then holds the total. A warp
+// of CTA `rank` calls it with its columns' place (`col` of the tile, lane `row`).
+// False with *ok = false when a wait gave up.
+template <int P, int BN, int CPT>
+__device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int row, int valid, float (&sum)[CPT],
+                                           bool *ok) {
+  const uint32_t turn = x.turn++;
+  if (rank) {
+    if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(x.empty, (turn & 1u) ^ 1u, WAIT_BUDGET))) {
+      *ok = false;
+      return false;
+    }
+    const uint32_t to = wgtc::mapa_shared(wgtc::smem_addr(x.buf + ((int)(rank - 1) * BN + col) * 128 + row), 0);
+#pragma unroll
+    for (int j = 0; j < CPT; j++)
+      if (j < valid) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 512u * j), "f"(sum[j]) : "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(x.full), 0));
+    return false;
+  }
+  if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(x.full, turn & 1u, WAIT_BUDGET))) {
+    *ok = false;
+    return false;
+  }
+#pragma unroll
+  for (int r = 0; r < P - 1; r++) {
+    const float *from = x.buf + (r * BN + col) * 128 + row;
+#pragma unroll
+    for (int j = 0; j < CPT; j++)
+      if (j < valid) sum[j] += from[128 * j];
+  }
+  __syncwarp();
+  const int lane = threadIdx.x & 31;
+  if (lane > 0 && lane < P) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(x.empty), (uint32_t)lane));
+  return true;
 }
 
 // A place in a ring of N stages, and the parity of the round it is in.
@@ -246,9 +309,10 @@ __device__ __forceinline__ uint32_t pair_rank() {
   if constexpr (CG == 2) return wgtc::cluster_ctarank();
   else return 0;
 }
-template <int CG>
-__device__ __forceinline__ void pair_sync() {
-  if constexpr (CG == 2) wgtc::cluster_sync();
+// All threads of a cluster of N CTAs meet.
+template <int N>
+__device__ __forceinline__ void cluster_sync() {
+  if constexpr (N > 1) wgtc::cluster_sync();
   else __syncthreads();
 }
 // One arrival on the leader's copy of `bar`. What it signals for a pair is that

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
     }
   };
   int r = warp;
-  if (wide) {
+  if (wide)
     for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
       Eight<T> w[ROWS_AT_ONCE];
 #pragma unroll
@@ -190,17 +190,27 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
 #pragma unroll
       for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) round(w[u], dst, r + 8 * u);
     }
-  }
-  for (; r < t.n; r += 8, src += src_step, dst += dst_step) {
-    Eight<T> w;
-    if (wide) {
+  // The rest, and lines that wide loads cannot read: lines past the end are read
+  // as the last one, so that these loads go out together too.
+  for (; r < t.n; r += 8 * ROWS_AT_ONCE) {
+    Eight<T> w[ROWS_AT_ONCE];
+    const int last = (t.n - 1 - r) >> 3;
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; i++) w.w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
-    } else {
+    for (int u = 0; u < ROWS_AT_ONCE; u++) {
+      const T *p = src + min(u, last) * src_step;
+      if (wide) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) w.v[i] = i < valid ? src[i] : T(0.0f);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[u].v[i] = i < valid ? p[i] : T(0.0f);
+      }
     }
-    round(w, dst, r);
+#pragma unroll
+    for (int u = 0; u < ROWS_AT_ONCE; u++)
+      if (u <= last) round(w[u], dst + u * dst_step, r + 8 * u);
+    src += ROWS_AT_ONCE * src_step;
+    dst += ROWS_AT_ONCE * dst_step;
   }
   __syncthreads();
   // (the second tile exists unless the tile row has an odd number of them)
@@ -353,7 +363,15 @@ __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
 #pragma unroll
       for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) store(code[u], dst, r + 8 * u);
     }
-    for (; r < t.n; r += 8, src += src_step, dst += dst_step) store(load(src), dst, r);
+    if (r < t.n) {
+      const int last = (t.n - 1 - r) >> 3;
+      uint32_t code[ROWS_AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++) code[u] = load(src + min(u, last) * src_step);
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++)
+        if (u <= last) store(code[u], dst + u * dst_step, r + 8 * u);
+    }
   }
 }
 
@@ -403,10 +421,7 @@ struct Args {
   int tiles_l;
   int l_atoms;           // scale tile rows of one matrix of B
   const int *offsets;    // NULL: one group, all rows
-  float alpha, beta;
-  void *C;
-  int64_t ldc;
-  int ctype;
+  wgg::Out out;
   unsigned *dwords;
 };
 
@@ -519,12 +534,12 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   wg_pdl_trigger();
   wgg::plan_groups(a.offsets, a.groups, a.rows, S::BN, start, tile0, atom0, a.dwords);
   wgtc::tc_fence_before();
-  wgg::pair_sync<CG>();
+  wgg::cluster_sync<CG>();
   wgtc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int64_t tiles = (int64_t)tile0[a.groups] * a.tiles_l;
   const int64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
-  const int kt = a.alpha == 0.0f ? 0 : (a.k + BKE - 1) / BKE;
+  const int kt = a.out.alpha == 0.0f ? 0 : (a.k + BKE - 1) / BKE;
   auto gave_up = [&](unsigned bit) {
     atomicOr(a.dwords + WG_DW_ERROR, bit);
     *abort_flag = 1;
@@ -633,7 +648,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       const Tile x = tile_at<S>(a, t, start, tile0, atom0);
       const int valid = x.nv - h * S::CPT;  // columns this warp has (may be none)
       const int l = x.l0 + (int)rank * BL + q * 32 + lane;
-      const int64_t at = (int64_t)(x.r0 + h * S::CPT) * a.ldc + l;
+      const int64_t at = (int64_t)(x.r0 + h * S::CPT) * a.out.ldc + l;
       const uint32_t col = tmem + (uint32_t)(h * S::CPT) + ((uint32_t)(q * 32) << 16);
       float sum[S::CPT];
 #pragma unroll
@@ -652,13 +667,13 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         __syncwarp();
         if (lane == 0) wgg::leader_arrive<CG>(&acc_empty[b]);
       }
-      if (ok && l < a.n) wgg::store_all<S::CPT>(a.C, a.ctype, at, a.ldc, valid, a.alpha, a.beta, sum);
+      if (ok) wgg::store_sums<S::CPT, SUMS>(a.out, at, l < a.n, valid, sum);
     }
   }
 
   wgtc::tc_fence_before();
   __syncwarp();
-  wgg::pair_sync<CG>();
+  wgg::cluster_sync<CG>();
   if (warp == 1) {
     wgtc::tc_fence_after();
     wgg::pair_tmem_dealloc<CG>(tmem, S::TMEM_COLS);
@@ -734,7 +749,7 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
   CUtensorMap m[4];
   memset(m, 0, sizeof m);
   a.tiles_l = (a.n + S::TL - 1) / S::TL;
-  if (a.alpha != 0.0f) {
+  if (a.out.alpha != 0.0f) {
     const cuuint64_t pitch = (cuuint64_t)pitch_of(a.k), words = (cuuint64_t)tiles_of(a.k) * 128;
     const cuuint64_t dl[3] = {pitch, (cuuint64_t)a.n, (cuuint64_t)a.groups}, sl[2] = {pitch, pitch * (cuuint64_t)a.n};
     const cuuint32_t bl[3] = {128, (cuuint32_t)BL, 1};
@@ -751,7 +766,7 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
         !encode(&m[2], u32, o.Bs, 2, dsl, &ss, bsl, no) || !encode(&m[3], u32, o.As, 2, dsn, &ss, bsn, no))
       return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
   }
-  return a.ctype == WG_TYPE_F32 && a.k > SEG * BKE ? launch_as<S, true>(d, family, a, m)
+  return a.out.type == WG_TYPE_F32 && a.k > SEG * BKE ? launch_as<S, true>(d, family, a, m)
                                                    : launch_as<S, false>(d, family, a, m);
 }
 
@@ -787,11 +802,7 @@ wg_status mx_gemm(wg_device *d, const char *family, int ctype, int64_t groups, i
   a.k = (int)k;
   a.l_atoms = (int)tiles_of(n);
   a.offsets = offsets;
-  a.alpha = alpha;
-  a.beta = beta;
-  a.C = C;
-  a.ldc = ldc;
-  a.ctype = ctype;
+  a.out = {C, ldc, alpha, beta, ctype};
   a.dwords = d->dwords;
   const Operands o = {static_cast<const uint8_t *>(A), static_cast<const uint8_t *>(As),
                       static_cast<const uint8_t *>(B), static_cast<const uint8_t *>(Bs)};
