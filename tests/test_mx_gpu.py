@@ -185,6 +185,14 @@ def test_gemm_pairs(wg, device, m, n, k, ctype):
     test_gemm(wg, device, m, n, k, ctype)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 200, 4096), (20, 1000, 8192), (33, 260, 3000), (64, 520, 5000), (100, 136, 2048),
+                                   (5, 8192, 1024), (40, 8192, 1100)])
+@pytest.mark.parametrize("ctype", ["float32", "bfloat16"])
+def test_gemm_few_rows(wg, device, m, n, k, ctype):
+    """Narrow tiles, and contractions split over several CTAs."""
+    test_gemm(wg, device, m, n, k, ctype)
+
+
 @pytest.mark.parametrize("m,n,k", [(64, 130, 9000), (2570, 2050, 4500)])
 def test_gemm_long(wg, device, m, n, k):
     test_gemm(wg, device, m, n, k, "float32")
@@ -252,6 +260,12 @@ def test_gemm_grouped(wg, device, sizes, first, after, n, k):
     gc.assert_close(values(wg, C).reshape(m, n), want, mag, k, 0.5, c0.astype(np.float64), "float32", "C")
     for x in (a, b, W, C, off):
         x.destroy()
+
+
+@pytest.mark.parametrize("sizes", [[3], [40, 0, 70], [1] * 9, [17] * 12, [130, 5]], ids=lambda s: f"{len(s)}g{sum(s)}")
+@pytest.mark.parametrize("n,k", [(264, 4096), (1000, 1100)])
+def test_gemm_grouped_few_rows(wg, device, sizes, n, k):
+    test_gemm_grouped(wg, device, sizes, 1, 2, n, k)
 
 
 @pytest.mark.parametrize("n,k", [(2048, 128), (2050, 600)])

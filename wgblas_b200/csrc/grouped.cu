@@ -573,7 +573,16 @@ wg_status launch(wg_device *d, Args &a, int type) {
 // SMs; a round takes its k-blocks times the larger of the tensor core's time and
 // the time an SM needs to receive the block (65 bytes a clock from L2), or the
 // clocks that issuing it takes; joining a split contraction adds a fixed time.
-// Groups are taken to be evenly filled: the host does not know their sizes.
+// Groups are taken to be evenly filled: the host does not know their sizes. us in
+// a CUDA graph, operands in L2, m x n x k (groups), the chosen form's starred:
+//                           pair   128 columns   64      32     64/2    32/2    32/4
+//   4 x 512 x 4096 (8)      16.1      15.8      15.6    15.6    11.3    11.2     8.4*
+//   64 x 4096 x 4096 (1)    16.6      16.5      16.3    15.8    13.1    12.1*   18.5
+//   8 x 1024 x 2048 (8)     10.2      10.2      10.1     9.6    10.5     9.4*   15.1
+//   512 x 512 x 512 (1)      7.8       5.7       5.1     4.8*    7.0     6.3    12.8
+//   1024 x 1024 x 1024 (1)  10.3       7.7       7.1*   10.2    11.3    14.0    42.4
+//   1000 x 1024 x 776 (7)   10.4       8.9*     11.3    10.3    14.0    15.3    44.2
+//   2000 x 2048 x 2048 (8)  16.8*     20.8      32.6    51.0    36.8    59.6   173
 enum Form { PAIR_256, ONE_128, ONE_64, ONE_32, SPLIT_64, SPLIT_32_2, SPLIT_32_4, FORMS };
 template <int MODE>
 Form choose(const wg_device *d, const Args &a) {

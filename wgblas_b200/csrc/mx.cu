@@ -103,22 +103,54 @@ __device__ __forceinline__ uint32_t top_of(const Eight<T> &w) {
 struct TileRows {
   int r0, n, b;
 };
-// smem: start and atom0 tables of the groups (grouped matrices only).
-__device__ __forceinline__ TileRows rows_of_tile(const QuantArgs &a, int tile, int *tables) {
-  TileRows t;
-  if (a.offsets) {
-    int *start = tables, *atom0 = tables + a.groups + 1;
-    wgg::plan_groups(a.offsets, a.groups, a.rows, 128, start, atom0, nullptr, a.dwords);
-    t.b = 0;
-    if (tile >= atom0[a.groups]) {
-      t.r0 = t.n = 0;
-      return t;
+// Grouped matrices: every warp finds its tile's group by itself, 32 groups at a
+// time, from the same clamped, non-decreasing offsets as plan_groups makes (the
+// first CTA goes through them all and reports offsets that this changes).
+__device__ __forceinline__ TileRows grouped_rows(const QuantArgs &a, int tile) {
+  const int lane = threadIdx.x & 31;
+  const bool check = blockIdx.x == 0 && threadIdx.x < 32;
+  TileRows t = {0, 0, 0};
+  const int first = a.offsets[0];
+  int top = max(min(first, a.rows), 0), tiles = 0;
+  bool bad = first != top, found = false;
+  for (int base = 0; base < a.groups && (!found || check); base += 32) {
+    const int j = base + lane;
+    const int raw = j < a.groups ? a.offsets[j + 1] : 0;
+    int end = max(min(raw, a.rows), 0);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) end = max(end, o);
     }
-    const int g = wgg::group_of(atom0, a.groups, tile);
-    t.r0 = start[g] + (tile - atom0[g]) * 128;
-    t.n = min(128, start[g + 1] - t.r0);
-    return t;
+    end = max(end, top);
+    bad |= j < a.groups && end != raw;
+    int start = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) start = top;
+    const int mine = (end - start + 127) >> 7;  // (0 past the last group: end stays)
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    sum += tiles;
+    const uint32_t hit = __ballot_sync(0xffffffffu, tile < sum);
+    if (hit && !found) {
+      const int f = __ffs(hit) - 1;
+      const int s0 = __shfl_sync(0xffffffffu, start, f), e0 = __shfl_sync(0xffffffffu, end, f);
+      t.r0 = s0 + (tile - __shfl_sync(0xffffffffu, sum - mine, f)) * 128;
+      t.n = min(128, e0 - t.r0);
+      found = true;
+    }
+    top = __shfl_sync(0xffffffffu, end, 31);
+    tiles = __shfl_sync(0xffffffffu, sum, 31);
   }
+  if (check && bad) atomicOr(a.dwords + WG_DW_ERROR, WG_DERR_OFFSETS);
+  return t;
+}
+__device__ __forceinline__ TileRows rows_of_tile(const QuantArgs &a, int tile) {
+  if (a.offsets) return grouped_rows(a, tile);
+  TileRows t;
   t.b = tile / a.tiles_r;
   t.r0 = (tile - t.b * a.tiles_r) * 128;
   t.n = min(128, a.rows - t.r0);
@@ -143,13 +175,12 @@ constexpr int ROWS_AT_ONCE = 4;  // a warp's loads in flight
 // figures at launch_quant.
 template <class T>
 __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
-  extern __shared__ int tables[];
   __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
   const int pairs = (a.tiles_c + 1) >> 1;
   const int tile = (int)(blockIdx.x / (unsigned)pairs), tc = (int)(blockIdx.x % (unsigned)pairs) * 2;
-  const TileRows t = rows_of_tile(a, tile, tables);
+  const TileRows t = rows_of_tile(a, tile);
   if (t.n <= 0) return;
   reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = 0;
   __syncthreads();
@@ -231,7 +262,7 @@ __global__ void __launch_bounds__(256) mx_quantize_t(const QuantArgs a) {
   wg_pdl_wait();
   wg_pdl_trigger();
   const int tile = (int)(blockIdx.x / (unsigned)a.tiles_c), tc = (int)(blockIdx.x % (unsigned)a.tiles_c);
-  const TileRows t = rows_of_tile(a, tile, nullptr);
+  const TileRows t = rows_of_tile(a, tile);
   if (threadIdx.x < 128) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = 0;
   __syncthreads();
   const int blk = threadIdx.x >> 6, r = (threadIdx.x & 63) * 2, col = tc * 128 + blk * 32;
@@ -315,13 +346,12 @@ __device__ __forceinline__ void decode4(uint32_t code, float scale, float *y) {
 template <class T>
 __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
   constexpr int E = 16 / sizeof(T), PASSES = 8 / E;
-  extern __shared__ int tables[];
   __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
   const int pairs = (a.tiles_c + 1) >> 1;
   const int tile = (int)(blockIdx.x / (unsigned)pairs), tc = (int)(blockIdx.x % (unsigned)pairs) * 2;
-  const TileRows t = rows_of_tile(a, tile, tables);
+  const TileRows t = rows_of_tile(a, tile);
   if (t.n <= 0) return;
   if (threadIdx.x < 128 || tc + 1 < a.tiles_c) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = tile_scales(a, tile, tc)[threadIdx.x];
   __syncthreads();
@@ -386,7 +416,11 @@ __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
 // Forms: CTA pairs with 256 x 256 tiles for compute-bound calls (an MMA of 64
 // takes as long as a bf16 one of 16, so the bytes a tile needs from L2 a clock
 // are the same as there, and with them the reason for pairs), one CTA with
-// 128 x 128 tiles otherwise. A pair's accumulator and scales leave no room for a
+// 128 columns otherwise, or a cluster of such that splits the contraction; 32
+// columns where the call has no more rows. (Tiles begin at whole scale tiles, 128
+// rows, of their group: the address of an MMA's scales in TMEM cannot be any
+// column. 32-column tiles inside a scale tile, at an odd one, raised "misaligned
+// address".) A pair's accumulator and scales leave no room for a
 // second accumulator in TMEM: the epilogue drains it to registers at once and
 // stores from there while the next tile's MMAs run.
 
@@ -397,21 +431,28 @@ constexpr size_t SMEM_LIMIT = 227 * 1024;
 // truncate (grouped.cu).
 constexpr int SEG = 16;
 
-template <int CG_, int BN_>
+// CG CTAs (a pair or one) share a tile's lanes, P CTAs its contraction.
+template <int CG_, int BN_, int P_ = 1>
 struct Shape {
-  static constexpr int CG = CG_, BN = BN_;
+  static constexpr int CG = CG_, BN = BN_, P = P_, CLUSTER = CG * P;
+  static_assert(CG == 1 || P == 1, "a pair shares lanes or contraction, not both");
   static constexpr int TL = CG * BL, CPT = BN / 2;
-  static constexpr int NT = BN / 128;            // scale tiles of the N side (every CTA of a pair has all)
+  static constexpr int NT = BN > 128 ? BN / 128 : 1;  // scale tiles of the N side (every CTA of a pair has all)
+  static constexpr int NBOX = BN < 64 ? BN : 64;      // rows of one N-side box
   static constexpr int L_BYTES = BL * 128, N_BYTES = BN / CG * 128;
   static constexpr int SF_L = 1024, SF_N = NT * 1024;
   static constexpr int STAGE = L_BYTES + N_BYTES + SF_L + SF_N;
-  static constexpr int STAGES = (int)((SMEM_LIMIT - 14 * 1024) / STAGE);
+  static constexpr int PARTS = (P - 1) * BN * BL * 4;
+  static constexpr int STAGES = (int)((SMEM_LIMIT - 14 * 1024 - PARTS) / STAGE);
   // TMEM columns: accumulators, then two sets of scales (L: 2 x 4, N: 2 x 4 NT).
   static constexpr int ACCS = BN <= 128 ? 2 : 1;
   static constexpr int SF_COL = ACCS * BN, SF_SET = 8 + 8 * NT;
-  static constexpr int TMEM_COLS = 512;
+  static constexpr int TMEM_COLS = BN <= 32 ? 128 : 512;
+  static_assert(BN == 32 || BN % 128 == 0, "tiles begin at whole scale tiles");
   static_assert(SF_COL + 2 * SF_SET <= TMEM_COLS, "accumulators and scales must fit TMEM");
-  static constexpr size_t tables = (size_t)STAGES * STAGE + 256;
+  static constexpr size_t parts = (size_t)STAGES * STAGE;
+  static constexpr size_t bars = parts + PARTS;
+  static constexpr size_t tables = bars + 256;
   static constexpr size_t smem(int groups) { return 1024 + tables + 3 * ((size_t)groups + 1) * sizeof(int); }
   static constexpr int NMMA_STEP = 32;
 };
@@ -470,11 +511,12 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
 struct Tile {
   int g, l0, r0, nv;
   int n_atom;  // scale tile row of the tile's first row
+  int k_lo, k_hi;  // this CTA's k-blocks
 };
 
 template <class S>
 __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *start, const int *tile0,
-                                        const int *atom0) {
+                                        const int *atom0, int kt, uint32_t rank) {
   Tile x;
   const int q = (int)(t / a.tiles_l);
   x.g = wgg::group_of(tile0, a.groups, q);
@@ -485,6 +527,8 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
   x.r0 = start[x.g] + first;
   x.nv = min(S::BN, start[x.g + 1] - x.r0);
   x.n_atom = atom0[x.g] + first / 128;
+  x.k_lo = S::P > 1 ? (int)((int64_t)kt * rank / S::P) : 0;
+  x.k_hi = S::P > 1 ? (int)((int64_t)kt * (rank + 1) / S::P) : kt;
   return x;
 }
 
@@ -498,17 +542,18 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = wgtc::smem_addr(smem_raw);
   uint8_t *smem = smem_raw + ((1024 - (base & 1023)) & 1023);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + (size_t)STAGES * S::STAGE);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::bars);
   uint64_t *empty = full + STAGES;
   uint64_t *acc_full = empty + STAGES;  // [2]
   uint64_t *acc_empty = acc_full + 2;   // [2]
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  wgg::Parts parts = {reinterpret_cast<float *>(smem + S::parts), acc_empty + 2, acc_empty + 3, 0};
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 4);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *start = reinterpret_cast<int *>(smem + S::tables);
   int *tile0 = start + a.groups + 1, *atom0 = tile0 + a.groups + 1;
 
   const int warp = wgg::warp_index(), lane = threadIdx.x & 31;
-  const uint32_t rank = wgg::pair_rank<CG>();
+  const uint32_t rank = S::CLUSTER > 1 ? wgtc::cluster_ctarank() : 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
       wgtc::mbar_init(&full[s], 2);
@@ -518,6 +563,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       wgtc::mbar_init(&acc_full[b], 1);
       wgtc::mbar_init(&acc_empty[b], CG * EPI_WARPS);
     }
+    wgtc::mbar_init(parts.full, EPI_WARPS * (S::P > 1 ? S::P - 1 : 1));
+    wgtc::mbar_init(parts.empty, EPI_WARPS);
     *abort_flag = 0;
     wgtc::fence_barrier_init();
   }
@@ -534,11 +581,12 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   wg_pdl_trigger();
   wgg::plan_groups(a.offsets, a.groups, a.rows, S::BN, start, tile0, atom0, a.dwords);
   wgtc::tc_fence_before();
-  wgg::cluster_sync<CG>();
+  wgg::cluster_sync<S::CLUSTER>();
   wgtc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int64_t tiles = (int64_t)tile0[a.groups] * a.tiles_l;
-  const int64_t t_first = blockIdx.x / CG, t_step = gridDim.x / CG;
+  const int64_t t_first = blockIdx.x / S::CLUSTER, t_step = gridDim.x / S::CLUSTER;
+  const uint32_t half = CG == 2 ? rank : 0;  // which lanes and columns of a pair's tile
   const int kt = a.out.alpha == 0.0f ? 0 : (a.k + BKE - 1) / BKE;
   auto gave_up = [&](unsigned bit) {
     atomicOr(a.dwords + WG_DW_ERROR, bit);
@@ -552,27 +600,27 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     const bool l_side = warp == 0;
     const uint32_t lead = wgg::leader_addr<CG>(full);
     for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-      const Tile x = tile_at<S>(a, t, start, tile0, atom0);
-      const int half = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
-      const int boxes = (half + 63) / 64;
-      const int l0 = x.l0 + (int)rank * BL, r0 = x.r0 + (int)rank * half;
+      const Tile x = tile_at<S>(a, t, start, tile0, atom0, kt, rank);
+      const int cols = ((x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1)) / CG;  // columns this CTA loads
+      const int boxes = (cols + S::NBOX - 1) / S::NBOX;
+      const int l0 = x.l0 + (int)half * BL, r0 = x.r0 + (int)half * cols;
       const int sl = x.g * a.l_atoms + l0 / 128;
-      const uint32_t bytes = l_side ? (uint32_t)(S::L_BYTES + S::SF_L) : (uint32_t)(boxes * 8192 + S::SF_N);
-      for (int kb = 0; kb < kt; kb++, ring.next()) {
+      const uint32_t bytes = l_side ? (uint32_t)(S::L_BYTES + S::SF_L) : (uint32_t)(boxes * S::NBOX * 128 + S::SF_N);
+      for (int kb = x.k_lo; kb < x.k_hi; kb++, ring.next()) {
         const int s = ring.s;
         ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET));
         if (!ok) break;
         uint8_t *st = smem + (size_t)s * S::STAGE, *sf = st + S::L_BYTES + S::N_BYTES;
         const uint32_t at = lead + 8u * (uint32_t)s;
         if (wgg::elect()) {
-          if (rank == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
+          if (half == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
           // (what lies past the last scale tile, or past the matrix's rows, arrives as zeros)
           if (l_side) {
             wgg::load_3d<CG>(st, &map_l, &full[s], at, kb * 128, l0, x.g);
             wgg::load_2d<CG>(sf, &map_sl, &full[s], at, kb * 256, sl);
           } else {
             for (int b = 0; b < boxes; b++)
-              wgg::load_2d<CG>(st + S::L_BYTES + b * 8192, &map_n, &full[s], at, kb * 128, r0 + b * 64);
+              wgg::load_2d<CG>(st + S::L_BYTES + b * S::NBOX * 128, &map_n, &full[s], at, kb * 128, r0 + b * S::NBOX);
             wgg::load_2d<CG>(sf + S::SF_L, &map_sn, &full[s], at, kb * 256, x.n_atom);
           }
         }
@@ -584,7 +632,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     for (int i = 0; i < STAGES && ok; i++, ring.next())
       if (!wgtc::mbar_wait_bounded(&empty[ring.s], ring.round ^ 1u, WAIT_BUDGET)) break;
   } else if (warp == 1) {
-    if (rank == 0) {
+    if (half == 0) {
       // ---- MMA issuer ----
       wgg::Ring<STAGES> ring;
       int used = 0;
@@ -596,11 +644,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       const uint64_t desc_s0 = scales_desc(smem0 + S::L_BYTES + S::N_BYTES);
       bool ok = true;
       for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-        const Tile x = tile_at<S>(a, t, start, tile0, atom0);
+        const Tile x = tile_at<S>(a, t, start, tile0, atom0, kt, rank);
         const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
         const uint32_t idesc0 = idesc_mxf4(S::TL, nmma, 0), idesc2 = idesc_mxf4(S::TL, nmma, 2);
-        for (int kb0 = 0; kb0 < kt && ok; kb0 += segment, used++) {
-          const int b = used % S::ACCS, kb1 = min(kt, kb0 + segment);
+        for (int kb0 = x.k_lo; kb0 < x.k_hi && ok; kb0 += segment, used++) {
+          const int b = used % S::ACCS, kb1 = min(x.k_hi, kb0 + segment);
           const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
           ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used / S::ACCS) & 1u) ^ 1u, WAIT_BUDGET));
           wgtc::tc_fence_after();
@@ -645,15 +693,15 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     int used = 0;
     bool ok = true;
     for (int64_t t = t_first; t < tiles && ok; t += t_step) {
-      const Tile x = tile_at<S>(a, t, start, tile0, atom0);
+      const Tile x = tile_at<S>(a, t, start, tile0, atom0, kt, rank);
       const int valid = x.nv - h * S::CPT;  // columns this warp has (may be none)
-      const int l = x.l0 + (int)rank * BL + q * 32 + lane;
+      const int l = x.l0 + (int)half * BL + q * 32 + lane;
       const int64_t at = (int64_t)(x.r0 + h * S::CPT) * a.out.ldc + l;
       const uint32_t col = tmem + (uint32_t)(h * S::CPT) + ((uint32_t)(q * 32) << 16);
       float sum[S::CPT];
 #pragma unroll
       for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
-      for (int kb0 = 0; kb0 < kt; kb0 += SUMS ? SEG : 1 << 30, used++) {
+      for (int kb0 = x.k_lo; kb0 < x.k_hi; kb0 += SUMS ? SEG : 1 << 30, used++) {
         const int b = used % S::ACCS;
         ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_full[b], (uint32_t)(used / S::ACCS) & 1u, WAIT_BUDGET) &&
                                          *abort_flag == 0);
@@ -662,18 +710,28 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
           break;
         }
         wgtc::tc_fence_after();
-        wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == 0, sum);
+        wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == x.k_lo, sum);
         wgtc::tc_fence_before();
         __syncwarp();
         if (lane == 0) wgg::leader_arrive<CG>(&acc_empty[b]);
       }
-      if (ok) wgg::store_sums<S::CPT, SUMS>(a.out, at, l < a.n, valid, sum);
+      if (!ok) break;
+      bool mine = true;
+      if constexpr (S::P > 1) {
+        if (kt) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, sum, &ok);
+        else mine = rank == 0;
+        if (!ok) {
+          if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
+          break;
+        }
+      }
+      if (mine) wgg::store_sums<S::CPT, SUMS && S::P == 1>(a.out, at, l < a.n, valid, sum);
     }
   }
 
   wgtc::tc_fence_before();
   __syncwarp();
-  wgg::cluster_sync<CG>();
+  wgg::cluster_sync<S::CLUSTER>();
   if (warp == 1) {
     wgtc::tc_fence_after();
     wgg::pair_tmem_dealloc<CG>(tmem, S::TMEM_COLS);
@@ -713,9 +771,8 @@ wg_status check_quant(const wg_device *d, int type, int64_t batch, int64_t rows,
 wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const QuantArgs), const QuantArgs &a, int ctas_a_row) {
   const int64_t tiles = a.offsets ? tiles_of(a.rows) + a.groups : (int64_t)a.batch * a.tiles_r;
   if (tiles * ctas_a_row >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
-  const size_t smem = a.offsets ? 2 * ((size_t)a.groups + 1) * sizeof(int) : 0;
   wg_launch_scope scope(d, family);
-  WG_CUDA(wg_launch_pdl(kern, dim3((unsigned)(tiles * ctas_a_row)), dim3(256), smem, d->stream, a));
+  WG_CUDA(wg_launch_pdl(kern, dim3((unsigned)(tiles * ctas_a_row)), dim3(256), 0, d->stream, a));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
 }
@@ -736,10 +793,10 @@ struct Operands {
 template <class S, bool SUMS>
 wg_status launch_as(wg_device *d, const char *family, Args &a, const CUtensorMap (&m)[4]) {
   const int64_t most = ((int64_t)a.rows / S::BN + a.groups) * a.tiles_l;
-  const unsigned grid = S::CG * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CG));
+  const unsigned grid = S::CLUSTER * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CLUSTER));
   wg_launch_scope scope(d, family);
   WG_CUDA(wg_kernel_smem(mx_gemm_kernel<S, SUMS>, SMEM_LIMIT));
-  WG_CUDA((wgg::launch<S::CG>(mx_gemm_kernel<S, SUMS>, grid, 352, S::smem(a.groups), d->stream, m[0], m[1], m[2], m[3], a)));
+  WG_CUDA((wgg::launch<S::CLUSTER>(mx_gemm_kernel<S, SUMS>, grid, 352, S::smem(a.groups), d->stream, m[0], m[1], m[2], m[3], a)));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
 }
@@ -754,7 +811,7 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
     const cuuint64_t dl[3] = {pitch, (cuuint64_t)a.n, (cuuint64_t)a.groups}, sl[2] = {pitch, pitch * (cuuint64_t)a.n};
     const cuuint32_t bl[3] = {128, (cuuint32_t)BL, 1};
     const cuuint64_t dn[2] = {pitch, (cuuint64_t)a.rows};
-    const cuuint32_t bn[2] = {128, 64};
+    const cuuint32_t bn[2] = {128, (cuuint32_t)S::NBOX};
     // Scales: rows of tiles, as 32-bit words; a box is two tiles long.
     const cuuint64_t ss = words * 4;
     const cuuint64_t dsl[2] = {words, (cuuint64_t)a.l_atoms * (cuuint64_t)a.groups};
@@ -766,8 +823,48 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
         !encode(&m[2], u32, o.Bs, 2, dsl, &ss, bsl, no) || !encode(&m[3], u32, o.As, 2, dsn, &ss, bsn, no))
       return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
   }
-  return a.out.type == WG_TYPE_F32 && a.k > SEG * BKE ? launch_as<S, true>(d, family, a, m)
-                                                   : launch_as<S, false>(d, family, a, m);
+  if constexpr (S::P > 1) return launch_as<S, true>(d, family, a, m);
+  else return a.out.type == WG_TYPE_F32 && a.k > SEG * BKE ? launch_as<S, true>(d, family, a, m)
+                                                          : launch_as<S, false>(d, family, a, m);
+}
+
+// The form with the least modelled time, as for the 16-bit products (grouped.cu);
+// joining parts costs about 3600 clocks, a pair's start and single accumulator
+// 3500. us in a CUDA graph, operands in L2, m x n x k (groups):
+//                            pair  128 columns  32 columns  ... split 2  split 4
+//   1024 x 4096 x 4096 (1)   12.2     13.0         -            -         -
+//   128 x 8192 x 4096 (1)    10.0      8.1         -            -         -
+//   1500 x 2048 x 4096 (32)  30.9     29.8         -            -         -
+//   16 x 8192 x 4096 (1)      7.4      6.6         6.3          6.7      11.8
+//   16 x 2048 x 8192 (1)     10.8      9.4         9.2          7.7       6.6
+//   30 x 2048 x 2048 (16)     9.8      9.3         7.8         12.1      33.2
+// (a split of 128-column tiles won nowhere by more than 4 % and is not built).
+// A 32-column form needs every group to fit it, which only the number of all rows can show here.
+enum Form { PAIR_256, ONE_128, ONE_32, SPLIT_32_2, SPLIT_32_4, FORMS };
+Form choose(const wg_device *d, const Args &a) {
+  static const struct { int cg, bn, p; } forms[FORMS] = {{2, 256, 1}, {1, 128, 1}, {1, 32, 1}, {1, 32, 2}, {1, 32, 4}};
+  const int64_t groups = std::max<int64_t>(1, std::min(a.groups, a.rows));
+  const int64_t cols = (a.rows + groups - 1) / groups, kt = std::max<int64_t>(1, (a.k + BKE - 1) / BKE);
+  Form best = ONE_128;
+  double least = 1e300;
+  for (int i = 0; i < FORMS; i++) {
+    const auto f = forms[i];
+    if (f.bn == 32 && a.rows > 32) continue;
+    const int64_t nt = (cols + f.bn - 1) / f.bn, nv = (cols + nt - 1) / nt;
+    const int64_t tl = (a.n + f.cg * BL - 1) / (f.cg * BL);
+    const int64_t slots = f.p == 4 ? d->sm_count * 3 / 16 : d->sm_count / (f.cg * f.p);
+    const int64_t rounds = (tl * groups * nt + slots - 1) / slots;
+    const int64_t box = std::min<int64_t>(f.bn, 64), lines = (nv / f.cg + box - 1) / box * box;
+    const double block = std::max({nv * 2.0, ((BL + lines) * 128 + 2048) / 65.0, 300.0});
+    const double tail = (double)BL * nv * (a.out.type == WG_TYPE_F32 ? 4 : 2) / 20 +
+                        (f.p > 1 ? 3600 : f.cg > 1 ? 3500 : 0);
+    const double t = rounds * (double)((kt + f.p - 1) / f.p) * block + tail;
+    if (t < least) {
+      least = t;
+      best = (Form)i;
+    }
+  }
+  return best;
 }
 
 wg_status mx_gemm(wg_device *d, const char *family, int ctype, int64_t groups, int64_t m, int64_t n, int64_t k,
@@ -807,9 +904,14 @@ wg_status mx_gemm(wg_device *d, const char *family, int ctype, int64_t groups, i
   const Operands o = {static_cast<const uint8_t *>(A), static_cast<const uint8_t *>(As),
                       static_cast<const uint8_t *>(B), static_cast<const uint8_t *>(Bs)};
   return wg_timed(d, gpu_ms, [&] {
-    const int64_t pairs = (n + 255) / 256 * std::max<int64_t>(groups, m / 256);
-    return m / groups > 128 && 2 * pairs >= d->sm_count ? launch_gemm<Shape<2, 256>>(d, family, a, o)
-                                                        : launch_gemm<Shape<1, 128>>(d, family, a, o);
+    const Form form = choose(d, a);
+    switch (form) {
+      case PAIR_256: return launch_gemm<Shape<2, 256>>(d, family, a, o);
+      case ONE_128: return launch_gemm<Shape<1, 128>>(d, family, a, o);
+      case ONE_32: return launch_gemm<Shape<1, 32>>(d, family, a, o);
+      case SPLIT_32_2: return launch_gemm<Shape<1, 32, 2>>(d, family, a, o);
+      default: return launch_gemm<Shape<1, 32, 4>>(d, family, a, o);
+    }
   });
 }
 
