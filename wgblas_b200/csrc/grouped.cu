@@ -59,10 +59,14 @@ struct Shape {
   static constexpr int PARTS = (P - 1) * BN * BL * 4;
   static constexpr int MAX_STAGES = 10;
   // Ring depth: what shared memory holds beside the groups' tables and the parts.
-  static constexpr int FIT = (int)((SMEM_LIMIT - 12 * 1024 - PARTS) / STAGE);
+  static constexpr int FIT = (int)((SMEM_LIMIT - 26 * 1024 - PARTS) / STAGE);
   static constexpr int STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
-  static constexpr int BARS = 4 * STAGES + 6;
-  static constexpr size_t parts = (size_t)STAGES * STAGE;
+  // Inner form: places for the last 16 lines of a group whose length is no
+  // multiple of 16, beside the ring (see the kernel).
+  static constexpr int ENDS = 2, END = (2 + (BN / CG + 63) / 64) * 2048;
+  static constexpr int BARS = 2 * STAGES + 4 * ENDS + 6;
+  static constexpr size_t ends = (size_t)STAGES * STAGE;
+  static constexpr size_t parts = ends + (size_t)ENDS * END;
   static constexpr size_t bars = parts + PARTS;
   static constexpr size_t tables = bars + (BARS * 8 + 8 + 15) / 16 * 16;
   static constexpr size_t smem(int groups) { return 1024 + tables + 2 * ((size_t)groups + 1) * sizeof(int); }
@@ -96,10 +100,10 @@ __device__ __forceinline__ uint32_t idesc_f16(uint32_t fmt, int M, int N, bool a
 }
 
 // Descriptor of an MN-major operand tile: 64-element (128-byte) chunks along
-// MN, CHUNK bytes apart (leading byte offset), each with its k lines 128 bytes
+// MN, `chunk` bytes apart (leading byte offset), each with its k lines 128 bytes
 // apart in groups of eight (stride byte offset 1024), 128-byte swizzle.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(CHUNK >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, int chunk = CHUNK) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(chunk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
 
@@ -128,8 +132,10 @@ struct Tile {
   int g, l0, n0, nv;
   int r0;     // rows form: the tile's first row; inner form: the group's first row
   int kt;     // k-blocks
-  int klen;   // contraction length
+  int klen;   // contraction length (inner form: without `end`)
   int k_lo, k_hi;  // this CTA's k-blocks
+  int end;    // inner form: lines past the last whole 16, when this CTA takes them
+  bool any;   // anything to contract
 };
 
 template <int MODE, class S>
@@ -163,30 +169,42 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
     x.nv = min(each, rows - first);
     x.klen = a.k;
   }
-  x.kt = a.out.alpha == 0.0f ? 0 : (x.klen + BK - 1) / BK;
+  if (a.out.alpha == 0.0f) x.klen = 0;
+  x.any = x.klen > 0;
+  x.end = 0;
+  if (MODE == INNER) {
+    if (rank % S::P == S::P - 1 || S::P == 1) x.end = x.klen & 15;
+    x.klen &= ~15;
+  }
+  x.kt = (x.klen + BK - 1) / BK;
   x.k_lo = S::P > 1 ? (int)((int64_t)x.kt * rank / S::P) : 0;
   x.k_hi = S::P > 1 ? (int)((int64_t)x.kt * (rank + 1) / S::P) : x.kt;
   return x;
 }
 
 // The lines past a group's last row hold the next group's (whatever they are,
-// infinities among them): zeroes those the last MMA of a k-block with `left`
-// lines would read, in `chunks` 64-element chunks. A whole warp calls it.
-__device__ __forceinline__ void zero_tail(uint8_t *st, int left, int chunks, int lane) {
-  const int end = (left + 15) & ~15;
+// infinities among them): zeroes lines `left` .. 15 of `chunks` 64-element chunks
+// of 16 lines. A whole warp calls it.
+__device__ __forceinline__ void zero_end(uint8_t *st, int left, int chunks, int lane) {
   for (int q = 0; q < chunks; q++)
-    for (int r = left + (lane >> 3); r < end; r += 4)
-      *reinterpret_cast<uint4 *>(st + q * CHUNK + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+    for (int r = left + (lane >> 3); r < 16; r += 4)
+      *reinterpret_cast<uint4 *>(st + q * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
   wgtc::fence_proxy_async_smem();
   __syncwarp();
 }
 
 // SUMS: accumulators are drained every SEG k-blocks (fp32 results).
 // Warps: 0 and 10 load (the L and the N side), 1 issues the MMAs, 2-9 store, 11
-// (inner form) zeroes what is past a group's last row.
+// (inner form) zeroes what is past a group's last row. That a group ends inside
+// the 16 lines of an MMA is known when its tile begins: those lines go to a place
+// of their own, loaded ahead of the tile's k-blocks and multiplied after them, so
+// that landing, zeroing and (in a pair) telling the other CTA are out of the way.
+// (With the last block zeroed in the ring they cost 27 us of 145 at 8192 rows in
+// 8 groups, 2048 x 4096 results.)
 template <int MODE, class S, bool SUMS>
 __global__ void __launch_bounds__(MODE == INNER ? 384 : 352, 1)
-grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n, const Args a) {
+grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n,
+               const __grid_constant__ CUtensorMap map_el, const __grid_constant__ CUtensorMap map_en, const Args a) {
   constexpr bool L_MN = MODE != ROWS_T, N_MN = MODE == INNER;
   constexpr int STAGES = S::STAGES, CG = S::CG;
   constexpr int NBOX = S::BN < 64 ? S::BN : 64;  // lines of one N-side box
@@ -195,9 +213,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   uint8_t *smem = smem_raw + ((1024 - (base & 1023)) & 1023);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::bars);
   uint64_t *empty = full + STAGES;
-  uint64_t *tail = empty + STAGES;       // inner form: this CTA's ragged last block has landed
-  uint64_t *tail_peer = tail + STAGES;   // ... and the other CTA of a pair has zeroed what is past its end
-  uint64_t *acc_full = tail_peer + STAGES;  // [2]
+  constexpr int ENDS = S::ENDS;
+  uint64_t *end_here = empty + STAGES;   // [ENDS] a group's last lines have landed in this CTA
+  uint64_t *end_peer = end_here + ENDS;  // ... the other CTA of a pair has zeroed what is past them
+  uint64_t *end_full = end_peer + ENDS;  // ... both have
+  uint64_t *end_empty = end_full + ENDS;
+  uint64_t *acc_full = end_empty + ENDS;    // [2]
   uint64_t *acc_empty = acc_full + 2;       // [2]
   wgg::Parts parts = {reinterpret_cast<float *>(smem + S::parts), acc_empty + 2, acc_empty + 3, 0};
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 4);
@@ -211,8 +232,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     for (int s = 0; s < STAGES; s++) {
       wgtc::mbar_init(&full[s], 2);
       wgtc::mbar_init(&empty[s], 1);
-      wgtc::mbar_init(&tail[s], 2);
-      wgtc::mbar_init(&tail_peer[s], 1);
+    }
+    for (int e = 0; e < ENDS; e++) {
+      wgtc::mbar_init(&end_here[e], 2);
+      wgtc::mbar_init(&end_peer[e], 1);
+      wgtc::mbar_init(&end_full[e], 1);
+      wgtc::mbar_init(&end_empty[e], 1);
     }
     for (int b = 0; b < 2; b++) {
       wgtc::mbar_init(&acc_full[b], 1);
@@ -248,6 +273,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
   if (warp == 0 || warp == 10) {
     // ---- producers: each CTA of a pair loads its own lanes and its half of the columns ----
     wgg::Ring<STAGES> ring;
+    wgg::Ring<ENDS> ends;
     bool ok = true;
     const bool l_side = warp == 0;
     const uint32_t lead = wgg::leader_addr<CG>(full);
@@ -259,6 +285,19 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       const int boxes = l_side ? 2 : (cols + NBOX - 1) / NBOX;
       const uint32_t bytes = (uint32_t)(l_side ? S::L_BYTES : boxes * NBOX * 128);
       const int lg = x.g * a.l_group;
+      if (MODE == INNER && x.end) {
+        const int e = ends.s;
+        ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&end_empty[e], ends.round ^ 1u, WAIT_BUDGET));
+        if (!ok) break;
+        if (wgg::elect()) {
+          uint8_t *dst = smem + S::ends + (size_t)e * S::END + (l_side ? 0 : 2 * 2048);
+          wgtc::mbar_arrive_expect_tx(&end_here[e], (uint32_t)boxes * 2048);
+          for (int b = 0; b < boxes; b++)
+            wgtc::tma_load_2d(dst + b * 2048, l_side ? &map_el : &map_en, &end_here[e], c0 + b * 64, x.r0 + x.klen);
+        }
+        __syncwarp();
+        ends.next();
+      }
       for (int kb = x.k_lo; kb < x.k_hi; kb++, ring.next()) {
         const int s = ring.s;
         ok = wgtc::mbar_wait_bounded(&empty[s], ring.round ^ 1u, WAIT_BUDGET);
@@ -268,28 +307,21 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         const int k0 = (MODE == INNER ? x.r0 : 0) + kb * BK;
         const uint32_t at = lead + 8u * (uint32_t)s;
         if (wgg::elect()) {
-          if (MODE == INNER && x.klen - kb * BK < BK && (x.klen & 15)) {
-            // A ragged end goes by way of warp 11.
-            wgtc::mbar_arrive_expect_tx(&tail[s], bytes);
-            for (int b = 0; b < boxes; b++)
-              wgtc::tma_load_2d(dst + b * CHUNK, l_side ? &map_l : &map_n, &tail[s], c0 + b * 64, k0);
-          } else {
-            if (half == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
-            if (l_side) {
-              if (MODE == ROWS_T) {
-                wgg::load_3d<CG>(dst, &map_l, &full[s], at, k0, c0, lg);
-              } else if (MODE == ROWS_N) {
-                wgg::load_3d<CG>(dst, &map_l, &full[s], at, c0, k0, lg);
-                wgg::load_3d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0, lg);
-              } else {
-                wgg::load_2d<CG>(dst, &map_l, &full[s], at, c0, k0);
-                wgg::load_2d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0);
-              }
+          if (half == 0) wgtc::mbar_arrive_expect_tx(&full[s], CG * bytes);
+          if (l_side) {
+            if (MODE == ROWS_T) {
+              wgg::load_3d<CG>(dst, &map_l, &full[s], at, k0, c0, lg);
+            } else if (MODE == ROWS_N) {
+              wgg::load_3d<CG>(dst, &map_l, &full[s], at, c0, k0, lg);
+              wgg::load_3d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0, lg);
             } else {
-              for (int b = 0; b < boxes; b++) {
-                if (N_MN) wgg::load_2d<CG>(dst + b * CHUNK, &map_n, &full[s], at, c0 + b * 64, k0);
-                else wgg::load_2d<CG>(dst + b * NBOX * 128, &map_n, &full[s], at, k0, c0 + b * NBOX);
-              }
+              wgg::load_2d<CG>(dst, &map_l, &full[s], at, c0, k0);
+              wgg::load_2d<CG>(dst + CHUNK, &map_l, &full[s], at, c0 + 64, k0);
+            }
+          } else {
+            for (int b = 0; b < boxes; b++) {
+              if (N_MN) wgg::load_2d<CG>(dst + b * CHUNK, &map_n, &full[s], at, c0 + b * 64, k0);
+              else wgg::load_2d<CG>(dst + b * NBOX * 128, &map_n, &full[s], at, k0, c0 + b * NBOX);
             }
           }
         }
@@ -301,41 +333,38 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
     // read a stage complete after its copies, and free it.
     for (int i = 0; i < STAGES && ok; i++, ring.next())
       if (!wgtc::mbar_wait_bounded(&empty[ring.s], ring.round ^ 1u, WAIT_BUDGET)) break;
+    for (int i = 0; i < ENDS && ok; i++, ends.next())
+      if (!wgtc::mbar_wait_bounded(&end_empty[ends.s], ends.round ^ 1u, WAIT_BUDGET)) break;
   } else if (MODE == INNER && warp == 11) {
-    // ---- ragged ends: zeroes the lines past a group's last row, then hands the stage on ----
-    int s = 0;
-    uint32_t phase = 0;  // parity of tail[s], tail_peer[s] at bit s
+    // ---- ragged ends: zeroes the lines past a group's last row, then hands the place on ----
+    wgg::Ring<ENDS> ends;
     for (int64_t t = t_first; t < tiles; t += t_step) {
       const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
-      if (x.k_hi == x.k_lo) continue;
-      s = (s + x.k_hi - x.k_lo - 1) % STAGES;  // this CTA's last block
-      const int left = x.klen - (x.k_hi - 1) * BK;  // (64 or more in front of another CTA's)
-      if (left < BK && (left & 15)) {
-        const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
-        bool ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&tail[s], phase >> s & 1u, WAIT_BUDGET));
-        if (ok) {
-          zero_tail(smem + (size_t)s * S::STAGE, left, 2 + (nmma / CG + 63) / 64, lane);
-          if (CG == 2 && half == 1) {
-            if (lane == 0) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(&tail_peer[s]), 0));
-          } else {
-            if (CG == 2)
-              ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(&tail_peer[s], phase >> s & 1u, WAIT_BUDGET));
-            if (ok && lane == 0)
-              asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(wgtc::smem_addr(&full[s])) : "memory");
-          }
+      if (!x.end) continue;
+      const int e = ends.s;
+      const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
+      bool ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&end_here[e], ends.round, WAIT_BUDGET));
+      if (ok) {
+        zero_end(smem + S::ends + (size_t)e * S::END, x.end, 2 + (nmma / CG + 63) / 64, lane);
+        if (CG == 2 && half == 1) {
+          if (lane == 0) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(&end_peer[e]), 0));
+        } else {
+          if (CG == 2)
+            ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(&end_peer[e], ends.round, WAIT_BUDGET));
+          if (ok && lane == 0) mbar_arrive(&end_full[e]);
         }
-        if (!ok) {
-          if (lane == 0) gave_up(WG_DERR_TMA_WAIT);
-          break;
-        }
-        phase ^= 1u << s;
       }
-      if (++s == STAGES) s = 0;
+      if (!ok) {
+        if (lane == 0) gave_up(WG_DERR_TMA_WAIT);
+        break;
+      }
+      ends.next();
     }
   } else if (warp == 1) {
     if (half == 0) {
       // ---- MMA issuer ----
       wgg::Ring<STAGES> ring;
+      wgg::Ring<ENDS> ends;
       int used = 0;
       constexpr int segment = SUMS ? SEG : 1 << 30;
       constexpr uint64_t step_l = (L_MN ? 2048 : 32) >> 4, step_n = (N_MN ? 2048 : 32) >> 4;
@@ -347,8 +376,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
         const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
         const uint32_t idesc = idesc_f16(a.ab_format, S::TL, nmma, L_MN, N_MN);
-        for (int kb0 = x.k_lo; kb0 < x.k_hi && ok; kb0 += segment, used++) {
+        if (x.k_hi == x.k_lo && !x.end) continue;
+        int kb0 = x.k_lo;
+        do {  // a segment (one without k-blocks when there is nothing but an end)
           const int b = used & 1, kb1 = min(x.k_hi, kb0 + segment);
+          const bool end = x.end && kb1 == x.k_hi;
           const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
           ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET));
           wgtc::tc_fence_after();
@@ -369,11 +401,26 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
                   mma_f16<CG>(d_tmem, dl + kk * step_l, dn + kk * step_n, idesc, kk > 0 || kb > kb0 ? 1u : 0u);
               }
               wgg::commit<CG>(&empty[ring.s]);
-              if (kb == kb1 - 1) wgg::commit<CG>(&acc_full[b]);
+              if (kb == kb1 - 1 && !end) wgg::commit<CG>(&acc_full[b]);
             }
             __syncwarp();
           }
-        }
+          if (MODE == INNER && ok && end) {
+            ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&end_full[ends.s], ends.round, WAIT_BUDGET));
+            if (!ok) break;
+            wgtc::tc_fence_after();
+            const uint32_t at = smem0 + (uint32_t)S::ends + (uint32_t)(ends.s * S::END);
+            if (wgg::elect()) {
+              mma_f16<CG>(d_tmem, smem_desc_mn(at, 2048), smem_desc_mn(at + 2 * 2048, 2048), idesc, kb1 > kb0 ? 1u : 0u);
+              wgg::commit<CG>(&end_empty[ends.s]);
+              wgg::commit<CG>(&acc_full[b]);
+            }
+            __syncwarp();
+            ends.next();
+          }
+          kb0 += segment;
+          used++;
+        } while (kb0 < x.k_hi && ok);
       }
       if (!ok && lane == 0) gave_up(WG_DERR_MMA_WAIT);
     }
@@ -406,7 +453,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         float sum[S::CPT];
 #pragma unroll
         for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
-        for (int kb0 = x.k_lo; kb0 < x.k_hi; kb0 += SUMS ? SEG : 1 << 30) {
+        for (int kb0 = x.k_lo; kb0 < x.k_hi || (kb0 == x.k_lo && x.end); kb0 += SUMS ? SEG : 1 << 30) {
           const int b = used & 1;
           if (!(ok = wait_acc(b))) break;
           wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == x.k_lo, sum);
@@ -415,7 +462,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         if (!ok) break;
         bool mine = true;
         if constexpr (S::P > 1) {
-          if (x.kt) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, sum, &ok);
+          if (x.any) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, sum, &ok);
           else mine = rank == 0;
           if (!ok) {
             if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
@@ -425,9 +472,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         if (mine) wgg::store_sums<S::CPT, SUMS && S::P == 1>(a.out, at, l < a.nl, valid, sum);
       } else {
         const int b = used & 1;
-        if (x.kt && !(ok = wait_acc(b))) break;
-        wgg::store_acc<S::CPT>(col + (uint32_t)(b * S::BN), x.kt != 0, a.out, at, l < a.nl, valid);
-        if (x.kt) free_acc(b);
+        if (x.any && !(ok = wait_acc(b))) break;
+        wgg::store_acc<S::CPT>(col + (uint32_t)(b * S::BN), x.any, a.out, at, l < a.nl, valid);
+        if (x.any) free_acc(b);
       }
     }
   }
@@ -523,12 +570,14 @@ bool mappable(const void *p, int64_t ld, int64_t stride) {
 
 // The tensor maps of a call (mappable operands).
 template <int MODE, class S>
-bool make_maps(const Args &a, int type, CUtensorMap *ml, CUtensorMap *mn) {
+bool make_maps(const Args &a, int type, CUtensorMap *ml, CUtensorMap *mn, CUtensorMap *el, CUtensorMap *en) {
   const cuuint64_t ldl = (cuuint64_t)a.ldl * 2, ldn = (cuuint64_t)a.ldn * 2;
   if (MODE == INNER) {
     const cuuint64_t dl[2] = {(cuuint64_t)a.nl, (cuuint64_t)a.rows}, dn[2] = {(cuuint64_t)a.nn, (cuuint64_t)a.rows};
     const cuuint32_t box[2] = {64, 64};
-    return encode(ml, type, a.L, 2, dl, &ldl, box) && encode(mn, type, a.N, 2, dn, &ldn, box);
+    const cuuint32_t end[2] = {64, 16};
+    return encode(ml, type, a.L, 2, dl, &ldl, box) && encode(mn, type, a.N, 2, dn, &ldn, box) &&
+           encode(el, type, a.L, 2, dl, &ldl, end) && encode(en, type, a.N, 2, dn, &ldn, end);
   }
   const int64_t lrows = MODE == ROWS_T ? a.nl : a.k, lcols = MODE == ROWS_T ? a.k : a.nl;
   const cuuint64_t dl[3] = {(cuuint64_t)lcols, (cuuint64_t)lrows, a.l_group ? (cuuint64_t)a.groups : 1};
@@ -540,7 +589,7 @@ bool make_maps(const Args &a, int type, CUtensorMap *ml, CUtensorMap *mn) {
 }
 
 template <int MODE, class S, bool SUMS>
-wg_status launch_as(wg_device *d, Args &a, const CUtensorMap &ml, const CUtensorMap &mn) {
+wg_status launch_as(wg_device *d, Args &a, const CUtensorMap (&m)[4]) {
   a.tiles_l = (a.nl + S::TL - 1) / S::TL;
   a.tiles_n = MODE == INNER ? (a.nn + S::BN - 1) / S::BN : 0;
   const int64_t most = (int64_t)a.tiles_l * (MODE == INNER ? (int64_t)a.groups * a.tiles_n
@@ -549,24 +598,23 @@ wg_status launch_as(wg_device *d, Args &a, const CUtensorMap &ml, const CUtensor
   wg_launch_scope scope(d, MODE == INNER ? "gemm_grouped_inner" : "gemm_grouped");
   WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, SUMS>, SMEM_LIMIT));
   WG_CUDA((wgg::launch<S::CLUSTER>(grouped_kernel<MODE, S, SUMS>, grid, MODE == INNER ? 384 : 352, S::smem(a.groups),
-                              d->stream, ml, mn, a)));
+                              d->stream, m[0], m[1], m[2], m[3], a)));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
 }
 
 template <int MODE, class S>
 wg_status launch(wg_device *d, Args &a, int type) {
-  CUtensorMap ml, mn;
-  memset(&ml, 0, sizeof ml);
-  memset(&mn, 0, sizeof mn);
+  CUtensorMap m[4];
+  memset(m, 0, sizeof m);
   // (no product, no operands)
-  if (a.out.alpha != 0.0f && !make_maps<MODE, S>(a, type, &ml, &mn))
+  if (a.out.alpha != 0.0f && !make_maps<MODE, S>(a, type, &m[0], &m[1], &m[2], &m[3]))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
   // One accumulator holds at most SEG k-blocks' sums of an fp32 result.
   // (a split contraction's sums are always drained, and few blocks long)
   const bool sums = S::P > 1 || (a.out.type == WG_TYPE_F32 && (MODE == INNER ? a.rows : a.k) > SEG * BK);
-  if constexpr (S::P > 1) return launch_as<MODE, S, true>(d, a, ml, mn);
-  else return sums ? launch_as<MODE, S, true>(d, a, ml, mn) : launch_as<MODE, S, false>(d, a, ml, mn);
+  if constexpr (S::P > 1) return launch_as<MODE, S, true>(d, a, m);
+  else return sums ? launch_as<MODE, S, true>(d, a, m) : launch_as<MODE, S, false>(d, a, m);
 }
 
 // The form with the least modelled time. A form's tiles run in rounds over the
