@@ -17,6 +17,7 @@
 // matrix whose rows are grouped, every group's scales begin at a new tile row.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "grouped_common.cuh"
 
@@ -210,25 +211,15 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
       if ((c & 3) == 0) sfb[(r & 31) * 16 + (r >> 5) * 4] = (uint8_t)e;
     }
   };
-  int r = warp;
-  if (wide)
-    for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
-      Eight<T> w[ROWS_AT_ONCE];
-#pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step)
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
-#pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) round(w[u], dst, r + 8 * u);
-    }
-  // The rest, and lines that wide loads cannot read: lines past the end are read
-  // as the last one, so that these loads go out together too.
-  for (; r < t.n; r += 8 * ROWS_AT_ONCE) {
-    Eight<T> w[ROWS_AT_ONCE];
+  // Lines past the end are read as the last one, so that a batch's loads go out
+  // together whatever its length.
+  auto batch = [&](auto count, int r, const T *from, uint8_t *to) {
+    constexpr int N = decltype(count)::value;
+    Eight<T> w[N];
     const int last = (t.n - 1 - r) >> 3;
 #pragma unroll
-    for (int u = 0; u < ROWS_AT_ONCE; u++) {
-      const T *p = src + min(u, last) * src_step;
+    for (int u = 0; u < N; u++) {
+      const T *p = from + min(u, last) * src_step;
       if (wide) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
@@ -238,11 +229,24 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < ROWS_AT_ONCE; u++)
-      if (u <= last) round(w[u], dst + u * dst_step, r + 8 * u);
-    src += ROWS_AT_ONCE * src_step;
-    dst += ROWS_AT_ONCE * dst_step;
-  }
+    for (int u = 0; u < N; u++)
+      if (u <= last) round(w[u], to + u * dst_step, r + 8 * u);
+  };
+  int r = warp;
+  if (wide && t.n > 64)
+    for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
+      Eight<T> w[ROWS_AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step)
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+#pragma unroll
+      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) round(w[u], dst, r + 8 * u);
+    }
+  // The rest (all of a short tile, at once), and lines that wide loads cannot read.
+  constexpr int REST = sizeof(T) == 2 ? 8 : 4;
+  for (; r < t.n; r += 8 * REST, src += REST * src_step, dst += REST * dst_step)
+    batch(std::integral_constant<int, REST>(), r, src, dst);
   __syncthreads();
   // (the second tile exists unless the tile row has an odd number of them)
   if (threadIdx.x < 128 || tc + 1 < a.tiles_c) tile_scales(a, tile, tc)[threadIdx.x] = reinterpret_cast<const uint32_t *>(sf)[threadIdx.x];
