@@ -398,10 +398,20 @@ cudaError_t launch(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t
 
 }  // namespace wgg
 
+// While it lives, this thread may make calls that set things up (a memory pool,
+// a kernel's attributes, its loading) although a stream is being captured: none
+// of them is work on that stream.
+struct wg_capture_relaxed {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  wg_capture_relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~wg_capture_relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Runs `queue` (which queues work on d->stream); on a handle opened with
 // WG_DEVICE_TIMING and with gpu_ms given, waits and reports its device time.
 template <class F>
 wg_status wg_timed(wg_device *d, float *gpu_ms, F queue) {
+  wg_capture_relaxed relaxed;
   if (!gpu_ms || !(d->flags & WG_DEVICE_TIMING)) return queue();
   WG_CUDA(cudaEventRecord(d->ev_start, d->stream));
   const wg_status st = queue();
