@@ -243,7 +243,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       wgtc::mbar_init(&acc_full[b], 1);
       wgtc::mbar_init(&acc_empty[b], CG * EPI_WARPS);
     }
-    wgtc::mbar_init(parts.full, EPI_WARPS * (S::P > 1 ? S::P - 1 : 1));
+    wgtc::mbar_init(parts.full, 1);
     wgtc::mbar_init(parts.empty, EPI_WARPS);
     *abort_flag = 0;
     wgtc::fence_barrier_init();
@@ -462,7 +462,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         if (!ok) break;
         bool mine = true;
         if constexpr (S::P > 1) {
-          if (x.any) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, sum, &ok);
+          if (x.any) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, x.nv,
+                                                                         warp == 2, sum, &ok);
           else mine = rank == 0;
           if (!ok) {
             if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
@@ -652,7 +653,7 @@ Form choose(const wg_device *d, const Args &a) {
     const double mma = nv * 2.0;  // 4 MMAs of 16: 2 clocks a column (128 or 256 lanes)
     const double block = std::max({mma, (BL + lines) * 128 / 65.0, 230.0});
     // A tile's results: the last round's are stored in the open (20 bytes a clock).
-    const double tail = (double)BL * nv * (a.out.type == WG_TYPE_F32 ? 4 : 2) / 20 + (f.p > 1 ? 2500 : 0);
+    const double tail = (double)BL * nv * (a.out.type == WG_TYPE_F32 ? 4 : 2) / 20 + (f.p > 1 ? 1800 : 0);
     const double t = rounds * (double)((kt + f.p - 1) / f.p) * block + tail;
     if (t < least) {
       least = t;

@@ -240,36 +240,43 @@ __device__ __forceinline__ void store_acc(uint32_t taddr, bool from, const Out &
 // P CTAs of a cluster share a tile, each with its part of the k-blocks; CTA 0
 // adds the others' sums to its own, in the order of their parts, and stores.
 // Their epilogue warps write them into its shared memory, [part][column][lane],
-// when its warps have read the last tile's.
+// when its warps have read the last tile's. The writes are asynchronous and count
+// themselves on CTA 0's barrier as they land, so nobody has to make them visible
+// (a release at cluster scope took about a thousand clocks).
 
 struct Parts {
   float *buf;        // CTA 0: (P - 1) x BN x 128 sums
-  uint64_t *full;    // CTA 0: the others' sums have arrived (8 warps x (P - 1) arrivals)
-  uint64_t *empty;   // others: CTA 0 has read them (8 arrivals)
+  uint64_t *full;    // CTA 0: the others' sums have arrived (one arrival and their bytes)
+  uint64_t *empty;   // others: CTA 0's warps have read them (8 arrivals)
   uint32_t turn;     // exchanges so far
 };
 
 // Joins sum[] over the cluster; true on CTA 0, which then holds the total. A warp
-// of CTA `rank` calls it with its columns' place (`col` of the tile, lane `row`).
+// of CTA `rank` calls it with its columns' place (`col` of the tile, lane `row`)
+// and the tile's number of columns; `first`: the one warp that announces the bytes.
 // False with *ok = false when a wait gave up.
 template <int P, int BN, int CPT>
-__device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int row, int valid, float (&sum)[CPT],
-                                           bool *ok) {
+__device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int row, int valid, int columns, bool first,
+                                           float (&sum)[CPT], bool *ok) {
   const uint32_t turn = x.turn++;
+  const int lane = threadIdx.x & 31;
   if (rank) {
-    if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(x.empty, (turn & 1u) ^ 1u, WAIT_BUDGET))) {
+    if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded(x.empty, (turn & 1u) ^ 1u, WAIT_BUDGET))) {
       *ok = false;
       return false;
     }
     const uint32_t to = wgtc::mapa_shared(wgtc::smem_addr(x.buf + ((int)(rank - 1) * BN + col) * 128 + row), 0);
+    const uint32_t bar = wgtc::mapa_shared(wgtc::smem_addr(x.full), 0);
 #pragma unroll
     for (int j = 0; j < CPT; j++)
-      if (j < valid) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 512u * j), "f"(sum[j]) : "memory");
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(x.full), 0));
+      if (j < valid)
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to + 512u * j),
+                     "r"(__float_as_uint(sum[j])), "r"(bar)
+                     : "memory");
     return false;
   }
-  if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(x.full, turn & 1u, WAIT_BUDGET))) {
+  if (first && lane == 0) wgtc::mbar_arrive_expect_tx(x.full, (uint32_t)((P - 1) * columns * BL * 4));
+  if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded(x.full, turn & 1u, WAIT_BUDGET))) {
     *ok = false;
     return false;
   }
@@ -281,8 +288,11 @@ __device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int
       if (j < valid) sum[j] += from[128 * j];
   }
   __syncwarp();
-  const int lane = threadIdx.x & 31;
-  if (lane > 0 && lane < P) wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(x.empty), (uint32_t)lane));
+  // (the sums are in registers: the arrival orders nothing else)
+  if (lane > 0 && lane < P)
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
+                     wgtc::mapa_shared(wgtc::smem_addr(x.empty), (uint32_t)lane))
+                 : "memory");
   return true;
 }
 

@@ -567,7 +567,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       wgtc::mbar_init(&acc_full[b], 1);
       wgtc::mbar_init(&acc_empty[b], CG * EPI_WARPS);
     }
-    wgtc::mbar_init(parts.full, EPI_WARPS * (S::P > 1 ? S::P - 1 : 1));
+    wgtc::mbar_init(parts.full, 1);
     wgtc::mbar_init(parts.empty, EPI_WARPS);
     *abort_flag = 0;
     wgtc::fence_barrier_init();
@@ -722,7 +722,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       if (!ok) break;
       bool mine = true;
       if constexpr (S::P > 1) {
-        if (kt) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, sum, &ok);
+        if (kt) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, x.nv,
+                                                              warp == 2, sum, &ok);
         else mine = rank == 0;
         if (!ok) {
           if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
@@ -833,7 +834,7 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
 }
 
 // The form with the least modelled time, as for the 16-bit products (grouped.cu);
-// joining parts costs about 3600 clocks, a pair's start and single accumulator
+// joining parts costs about 2400 clocks, a pair's start and single accumulator
 // 3500. us in a CUDA graph, operands in L2, m x n x k (groups):
 //                            pair  128 columns  32 columns  ... split 2  split 4
 //   1024 x 4096 x 4096 (1)   12.2     13.0         -            -         -
@@ -861,7 +862,7 @@ Form choose(const wg_device *d, const Args &a) {
     const int64_t box = std::min<int64_t>(f.bn, 64), lines = (nv / f.cg + box - 1) / box * box;
     const double block = std::max({nv * 2.0, ((BL + lines) * 128 + 2048) / 65.0, 300.0});
     const double tail = (double)BL * nv * (a.out.type == WG_TYPE_F32 ? 4 : 2) / 20 +
-                        (f.p > 1 ? 3600 : f.cg > 1 ? 3500 : 0);
+                        (f.p > 1 ? 2400 : f.cg > 1 ? 3500 : 0);
     const double t = rounds * (double)((kt + f.p - 1) / f.p) * block + tail;
     if (t < least) {
       least = t;
