@@ -360,6 +360,43 @@ def test_abi_refusals(wg, dev):
     assert b"NULL" in L.wg_last_error()
 
 
+def test_abi_refuses_what_is_not_aligned_to_its_elements(wg, dev):
+    """Every pointer of every entry point, one at a time; the kernels read and write whole elements."""
+    L, h = wg._native.lib, dev.handle
+    p, at1, at2 = (ct.c_void_p((1 << 20) + o) for o in (0, 1, 2))
+    f32, bf16 = wg._native.WG_TYPE_F32, wg._native.WG_TYPE_BF16
+    calls = [
+        (L.wg_gemm_grouped_dev, [h, bf16, bf16, 1, 2, 4, 4, 8, 1.0, p, 8, p, 8, 32, p, 0.0, p, 4, None],
+         [(9, at1), (11, at1), (14, at2), (16, at1)]),
+        (L.wg_gemm_grouped_inner_dev, [h, bf16, f32, 2, 4, 4, 8, 1.0, p, 8, p, 8, p, 0.0, p, 4, 16, None],
+         [(8, at1), (10, at1), (12, at2), (14, at2)]),
+        (L.wg_mx_quantize_dev, [h, bf16, 0, 1, 4, 40, p, 40, 0, 2, p, p, p, None], [(6, at1), (10, at2)]),
+        (L.wg_mx_quantize_dev, [h, f32, 1, 1, 4, 40, p, 40, 0, 0, None, p, p, None], [(6, at2)]),
+        (L.wg_mx_dequantize_dev, [h, f32, 1, 4, 40, p, p, 2, p, p, 40, 0, None], [(8, at1), (9, at2)]),
+        (L.wg_mx_gemm_dev, [h, f32, 4, 4, 64, 1.0, p, p, p, p, 0.0, p, 4, None], [(11, at2)]),
+        (L.wg_mx_gemm_grouped_dev, [h, bf16, 2, 4, 4, 64, 1.0, p, p, p, p, p, 0.0, p, 4, None], [(11, at2), (13, at1)]),
+    ]
+    for fn, ok, odd in calls:
+        assert fn(*ok) == wg._native.WG_ERR_NOT_SUPPORTED, fn.__name__
+        for i, v in odd:
+            a = list(ok)
+            a[i] = v
+            assert fn(*a) == wg._native.WG_ERR_INVALID_ARGUMENT, (fn.__name__, i)
+            assert b"aligned to its elements" in L.wg_last_error()
+
+
+def test_abi_strides_past_64_bits(wg, dev):
+    """Matrices that would overlap are refused also where rows * ld leaves 64 bits."""
+    L, bad, h = wg._native.lib, wg._native.WG_ERR_INVALID_ARGUMENT, dev.handle
+    p, ld = ct.c_void_p(1 << 20), (1 << 40) - 8
+    rows = (1 << 24) + 2  # (rows - 1) * ld is 2^64 and a little: 2^40 in 64 bits
+    assert L.wg_mx_dequantize_dev(h, 1, 2, rows, 40, p, p, 0, None, p, ld, (1 << 40) - 1, None) == bad
+    assert b"at least one matrix" in L.wg_last_error()
+    assert L.wg_gemm_grouped_inner_dev(h, 1, 0, 2, rows, 40, 8, 1.0, p, rows, p, 40, p, 0.0, p, ld, (1 << 40) - 1,
+                                       None) == bad
+    assert b"at least one matrix" in L.wg_last_error()
+
+
 # ---- conversions -----------------------------------------------------------------------
 
 

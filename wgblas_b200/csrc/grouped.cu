@@ -625,13 +625,13 @@ wg_status launch(wg_device *d, Args &a, int type) {
 // Groups are taken to be evenly filled: the host does not know their sizes. us in
 // a CUDA graph, operands in L2, m x n x k (groups), the chosen form's starred:
 //                           pair   128 columns   64      32     64/2    32/2    32/4
-//   4 x 512 x 4096 (8)      16.1      15.8      15.6    15.6    11.3    11.2     8.4*
-//   64 x 4096 x 4096 (1)    16.6      16.5      16.3    15.8    13.1    12.1*   18.5
-//   8 x 1024 x 2048 (8)     10.2      10.2      10.1     9.6    10.5     9.4*   15.1
-//   512 x 512 x 512 (1)      7.8       5.7       5.1     4.8*    7.0     6.3    12.8
-//   1024 x 1024 x 1024 (1)  10.3       7.7       7.1*   10.2    11.3    14.0    42.4
-//   1000 x 1024 x 776 (7)   10.4       8.9*     11.3    10.3    14.0    15.3    44.2
-//   2000 x 2048 x 2048 (8)  16.8*     20.8      32.6    51.0    36.8    59.6   173
+//   4 x 512 x 4096 (8)      16.0      15.9      15.6    15.6    10.8    10.7     7.8*
+//   64 x 4096 x 4096 (1)    16.6      16.6      16.3    15.9    12.8    11.6*   17.4
+//   8 x 1024 x 2048 (8)     10.2      10.3      10.1     9.6    10.6     8.9*   13.5
+//   512 x 512 x 512 (1)      7.8       5.7       5.0     4.9*    6.7     5.8    11.8
+//   1024 x 1024 x 1024 (1)  10.3       7.7       7.0*   10.2    10.2    12.6    28.1
+//   1000 x 1024 x 776 (7)   10.4       9.0*     11.2    10.4    12.6    13.2    29.4
+//   2000 x 2048 x 2048 (8)  16.6*     20.8      32.7    51.2    34.9    58.5   129
 enum Form { PAIR_256, ONE_128, ONE_64, ONE_32, SPLIT_64, SPLIT_32_2, SPLIT_32_4, FORMS };
 template <int MODE>
 Form choose(const wg_device *d, const Args &a) {
@@ -753,11 +753,12 @@ wg_status check_common(const wg_device *d, int type, int ctype, int64_t groups, 
   return WG_OK;
 }
 
-// Loads and stores go by elements of the operands' types.
-wg_status check_aligned(const void *A, const void *B, const void *C, int ctype) {
-  if (((uintptr_t)A | (uintptr_t)B) & 1 || ((uintptr_t)C & (ctype == WG_TYPE_F32 ? 3 : 1)))
-    return wg_fail(WG_ERR_INVALID_ARGUMENT, "A, B, and C must be aligned to their elements.");
-  return WG_OK;
+wg_status check_pointers(const void *A, const void *B, const void *C, int type, int ctype, const int *offsets) {
+  wg_status st;
+  if ((st = wgg::check_aligned("A", A, type)) != WG_OK || (st = wgg::check_aligned("B", B, type)) != WG_OK ||
+      (st = wgg::check_aligned("C", C, ctype)) != WG_OK)
+    return st;
+  return wgg::check_offsets(offsets);
 }
 
 wg_status check_ld(const char *name, int64_t ld, int64_t cols) {
@@ -786,7 +787,7 @@ extern "C" wg_status wg_gemm_grouped_dev(wg_device *d, int type, int ctype, int 
   if (groups == 0 || m == 0 || n == 0) return WG_OK;
   if (!offsets || !C || (k > 0 && alpha != 0.0f && (!A || !B)))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
-  if ((st = check_aligned(A, B, C, ctype)) != WG_OK) return st;
+  if ((st = check_pointers(A, B, C, type, ctype, offsets)) != WG_OK) return st;
   st = wgg::check_arch(d);
   if (st != WG_OK) return st;
   if (beta == 1.0f && (alpha == 0.0f || k == 0)) return WG_OK;  // C stays as it is
@@ -819,12 +820,12 @@ extern "C" wg_status wg_gemm_grouped_inner_dev(wg_device *d, int type, int ctype
       (st = check_ld("ldc", ldc, n)) != WG_OK)
     return st;
   // Each group writes its own matrix.
-  if (groups > 1 && (strideC < (m > 0 ? (m - 1) * ldc + n : 0) || strideC >= ((int64_t)1 << 40)))
+  if (groups > 1 && (strideC < 0 || !wgg::apart(strideC, m, n, ldc) || strideC >= ((int64_t)1 << 40)))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "strideC must be at least one matrix of C and below 2^40.");
   if (groups == 0 || m == 0 || n == 0) return WG_OK;
   if (!offsets || !C || (k > 0 && alpha != 0.0f && (!A || !B)))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
-  if ((st = check_aligned(A, B, C, ctype)) != WG_OK) return st;
+  if ((st = check_pointers(A, B, C, type, ctype, offsets)) != WG_OK) return st;
   st = wgg::check_arch(d);
   if (st != WG_OK) return st;
   if (beta == 1.0f && (alpha == 0.0f || k == 0)) return WG_OK;  // C stays as it is

@@ -386,6 +386,21 @@ inline wg_status check_arch(const wg_device *d) {
   return WG_OK;
 }
 
+// A matrix's elements and the offsets are read and written by their own types.
+inline wg_status check_aligned(const char *name, const void *p, int type) {
+  if ((uintptr_t)p & (type == WG_TYPE_F32 ? 3 : 1))
+    return wg_fail(WG_ERR_INVALID_ARGUMENT, "%s must be aligned to its elements.", name);
+  return WG_OK;
+}
+inline wg_status check_offsets(const int *offsets) {
+  if ((uintptr_t)offsets & 3) return wg_fail(WG_ERR_INVALID_ARGUMENT, "offsets must be aligned to its elements.");
+  return WG_OK;
+}
+// Whether matrices `stride` elements apart lie one after the other.
+inline bool apart(int64_t stride, int64_t rows, int64_t cols, int64_t ld) {
+  return rows <= 0 || (__int128)stride >= (__int128)(rows - 1) * ld + cols;
+}
+
 // Launches a kernel over clusters of CG CTAs with programmatic stream
 // serialization (the kernel calls wg_pdl_wait before it touches memory).
 template <int CG, class... KArgs, class... Args>

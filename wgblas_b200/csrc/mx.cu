@@ -770,7 +770,7 @@ wg_status check_quant(const wg_device *d, int type, int64_t batch, int64_t rows,
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "groups must be at most %d.", WG_MAX_GROUPS);
   if (groups > 0 && (batch != 1 || !offsets))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "a matrix with grouped rows has batch 1 and offsets.");
-  return WG_OK;
+  return groups > 0 ? wgg::check_offsets(offsets) : WG_OK;
 }
 
 wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const QuantArgs), const QuantArgs &a, int ctas_a_row) {
@@ -892,6 +892,7 @@ wg_status mx_gemm(wg_device *d, const char *family, int ctype, int64_t groups, i
   if (!C) return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
   if (k == 0) alpha = 0.0f;
   wg_status st;
+  if ((st = wgg::check_aligned("C", C, ctype)) != WG_OK || (st = wgg::check_offsets(offsets)) != WG_OK) return st;
   if (alpha != 0.0f && ((st = check_matrix("A", A, As)) != WG_OK || (st = check_matrix("B", B, Bs)) != WG_OK)) return st;
   st = wgg::check_arch(d);
   if (st != WG_OK) return st;
@@ -936,7 +937,9 @@ extern "C" wg_status wg_mx_quantize_dev(wg_device *d, int type, int trans, int64
   if (ldx < (trans ? rows : cols)) return wg_fail(WG_ERR_INVALID_ARGUMENT, "ldx must be >= cols of X as stored.");
   if (batch == 0 || rows == 0 || cols == 0) return WG_OK;
   if (!X) return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
-  if ((st = check_matrix("out", codes, scales)) != WG_OK || (st = wgg::check_arch(d)) != WG_OK) return st;
+  if ((st = wgg::check_aligned("X", X, type)) != WG_OK || (st = check_matrix("out", codes, scales)) != WG_OK ||
+      (st = wgg::check_arch(d)) != WG_OK)
+    return st;
   if (batch >= LIM || batch * tiles_of(rows) >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
   wg_device_guard guard(d->ordinal);
   QuantArgs a = {X, ldx, strideX, type, (int)rows, (int)cols, static_cast<uint8_t *>(codes),
@@ -961,11 +964,13 @@ extern "C" wg_status wg_mx_dequantize_dev(wg_device *d, int type, int64_t batch,
   if (ldx <= 0 || ldx >= ((int64_t)1 << 40) || strideX < 0 || strideX >= ((int64_t)1 << 40))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "ldx must be positive, strideX non-negative, both below 2^40.");
   if (ldx < cols) return wg_fail(WG_ERR_INVALID_ARGUMENT, "ldx must be >= cols of X as stored.");
-  if (batch > 1 && rows > 0 && strideX < (rows - 1) * ldx + cols)
+  if (batch > 1 && !wgg::apart(strideX, rows, cols, ldx))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "strideX must be at least one matrix of X.");
   if (batch == 0 || rows == 0 || cols == 0) return WG_OK;
   if (!X) return wg_fail(WG_ERR_INVALID_ARGUMENT, "operand pointer is NULL");
-  if ((st = check_matrix("X", codes, scales)) != WG_OK || (st = wgg::check_arch(d)) != WG_OK) return st;
+  if ((st = wgg::check_aligned("X", X, type)) != WG_OK || (st = check_matrix("x", codes, scales)) != WG_OK ||
+      (st = wgg::check_arch(d)) != WG_OK)
+    return st;
   if (batch >= LIM || batch * tiles_of(rows) >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
   wg_device_guard guard(d->ordinal);
   QuantArgs a = {X, ldx, strideX, type, (int)rows, (int)cols, static_cast<uint8_t *>(const_cast<void *>(codes)),
