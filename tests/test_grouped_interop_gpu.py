@@ -262,6 +262,26 @@ def test_results_past_two_to_the_31_elements(wg, dev):
         check(y[r], want, mag, k, "bfloat16")
 
 
+def test_as_many_rows_as_a_call_takes(wg, dev):
+    m, n, k = (1 << 31) - 1025, 8, 8
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 70 GB of free device memory")
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+    spots = [slice(0, 500), slice(1 << 30, (1 << 30) + 300), slice(m - 700, m)]
+    for r in spots:
+        x[r] = torch.randn((r.stop - r.start, k), device="cuda").to(torch.bfloat16)
+    w = torch.randn((2, n, k), device="cuda").to(torch.bfloat16)
+    forward(wg, dev, x, w, offsets_of([m - 5, 5]), y)
+    dev.check()
+    for r in spots:
+        last = 5 if r.stop == m else 0
+        want, mag = rows64(x[r], w, torch.tensor([0, r.stop - r.start - last, r.stop - r.start]))
+        check(y[r], want, mag, k, "bfloat16")
+    del x, y
+    torch.cuda.empty_cache()
+
+
 def test_weights_past_two_to_the_31_elements(wg, dev):
     groups, n, k = 40, 8192, 8192
     w = torch.zeros((groups, n, k), dtype=torch.bfloat16, device="cuda")
@@ -305,6 +325,22 @@ def test_full_size(wg, dev):
         if sizes[g]:  # sums are drained: what truncation leaves is far below the bound
             e = (dw[g].double() - a.t() @ b).norm() / (a.t() @ b).norm()
             assert e < 1e-6
+
+
+def test_full_size_in_4_bits(wg, dev):
+    m, n, k = 4096, 8192, 4096
+    x, w, off = make([m], n, k)
+    xq, wq = wg.GpuMxMatrix.empty(dev, m, k), wg.GpuMxMatrix.empty(dev, n, k)
+    wg.mxQuantize(dev, N, m, k, x, k, xq)
+    wg.mxQuantize(dev, N, n, k, w, k, wq)
+    y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    wg.mxGemm(dev, m, n, k, 1.0, xq, wq, 0.0, y, n)
+    xv, wv = torch.empty((m, k), device="cuda"), torch.empty((n, k), device="cuda")
+    wg.mxDequantize(dev, xq, xv, k)
+    wg.mxDequantize(dev, wq, wv, k)
+    want, mag = rows64(xv, wv[None], off)
+    check(y, want, mag, k, "bfloat16")
+    xq.destroy(), wq.destroy()
 
 
 # ---- together ------------------------------------------------------------------------------------

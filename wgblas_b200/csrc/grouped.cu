@@ -162,7 +162,7 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
     // The group's rows are divided evenly among its tiles: a last tile of a few
     // rows would load as many weights as a full one.
     const int rows = start[x.g + 1] - start[x.g];
-    const int each = ((rows + ntok - 1) / ntok + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
+    const int each = ((rows - 1) / ntok + S::NMMA_STEP) & ~(S::NMMA_STEP - 1);
     const int first = (local % ntok) * each;
     x.r0 = start[x.g] + first;
     x.n0 = first;
