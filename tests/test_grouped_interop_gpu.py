@@ -218,6 +218,36 @@ def test_two_streams_with_unaligned_operands(wg, dev):
         check(y, want, mag, 1501, "float32")
 
 
+def test_threads_with_unaligned_operands(wg, dev):
+    """Threads share a handle: each call's aligned copies stay with its own product."""
+    import threading
+
+    cases = [make([300 + i, 200], 257 + 2 * i, 1001 + 2 * i, torch.bfloat16, i) for i in range(4)]
+    outs = [torch.zeros((500 + i, 257 + 2 * i), device="cuda") for i in range(4)]
+    torch.cuda.synchronize()
+    start, errors = threading.Barrier(4), []
+
+    def work(i):
+        try:
+            start.wait()
+            for _ in range(50):
+                forward(wg, dev, *cases[i], outs[i])
+        except Exception as e:  # noqa: BLE001 (reported below)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    torch.cuda.synchronize()
+    dev.check()
+    for (x, w, off), y in zip(cases, outs):
+        want, mag = rows64(x, w, off)
+        check(y, want, mag, x.shape[1], "float32")
+
+
 # ---- values that must not spread ----------------------------------------------------------
 
 

@@ -434,9 +434,13 @@ struct wg_capture_relaxed {
 
 // Runs `queue` (which queues work on d->stream); on a handle opened with
 // WG_DEVICE_TIMING and with gpu_ms given, waits and reports its device time.
+// Calls on one handle from several threads queue one after the other: a call's
+// copies in the handle's temporary memory and the product that reads them must
+// be neighbours on the stream, and the handle's events are one pair.
 template <class F>
 wg_status wg_timed(wg_device *d, float *gpu_ms, F queue) {
   wg_capture_relaxed relaxed;
+  std::lock_guard<std::mutex> turn(d->queueing);
   if (!gpu_ms || !(d->flags & WG_DEVICE_TIMING)) return queue();
   WG_CUDA(cudaEventRecord(d->ev_start, d->stream));
   const wg_status st = queue();

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -95,6 +96,7 @@ struct wg_device {
   size_t flow_flags_n;
   uint32_t flow_epoch;
   cudaStream_t h2d, d2h;  // copy streams of the host-array path (created on first use)
+  std::mutex queueing;  // held while a grouped or microscaled call queues its work (wg_timed)
   void *temp;         // memory wg_temp_get keeps, last used on temp_stream
   size_t temp_bytes;
   cudaStream_t temp_stream;
