@@ -316,6 +316,16 @@ def test_mx_gemm_checks(wg, dev):
     assert wg.mxGemmGrouped(*{**grouped, "groups": 0}.values()) == {}
 
 
+def test_codes_and_scales_in_the_same_memory_are_refused(wg, dev):
+    codes, scales = wg.mxCodesSize(40, 50), wg.mxScalesSize(40, 50)
+    c = Tensor(codes, "uint8", at(0))
+    for where in (at(0), at(0) + codes - 16, at(0) - scales + 16):
+        with pytest.raises(wg.Error, match="codes must not overlap scales"):
+            wg.GpuMxMatrix.wrap(dev, c, Tensor(scales, "uint8", where), 40, 50)
+    for where in (at(0) + codes, at(0) - scales):
+        wg.GpuMxMatrix.wrap(dev, c, Tensor(scales, "uint8", where), 40, 50)
+
+
 # ---- C ABI -------------------------------------------------------------------------
 
 

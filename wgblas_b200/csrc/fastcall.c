@@ -410,7 +410,9 @@ static PyObject *mx_wrap(PyObject *self, PyObject *const *v, Py_ssize_t nv) {
       groups > WG_MAX_GROUPS || (groups && batch != 1) || !get_operand(&d, v[1], &c) || !get_operand(&d, v[2], &s))
     Py_RETURN_NONE;
   const int64_t nc = codes_size(rows, cols, batch), ns = scales_size(rows, cols, batch, groups);
-  if (c.type != T_U8 || s.type != T_U8 || nc < 0 || ns < 0 || c.n < nc || s.n < ns || ((c.p | s.p) & 15)) Py_RETURN_NONE;
+  if (c.type != T_U8 || s.type != T_U8 || nc < 0 || ns < 0 || c.n < nc || s.n < ns || ((c.p | s.p) & 15) ||
+      !apart(c.p, nc, s.p, ns))
+    Py_RETURN_NONE;
   PyTypeObject *t = (PyTypeObject *)t_mx;
   PyObject *x = t->tp_alloc(t, 0);
   if (!x) return NULL;

@@ -61,6 +61,8 @@ class GpuMxMatrix:
             raise Error("codes and scales must be uint8.")
         need("codes", nc, mxCodesSize(rows, cols, batch), "rows, cols, and batch")
         need("scales", ns, mxScalesSize(rows, cols, batch, groups), "rows, cols, batch, and groups")
+        disjoint("codes", (self._codes, mxCodesSize(rows, cols, batch)), tc,
+                 (("scales", self._scales, mxScalesSize(rows, cols, batch, groups), ts),))
         if (self._codes | self._scales) & 15:
             raise Error("codes and scales must be 16-byte aligned.")
 
