@@ -4,7 +4,11 @@ The public names follow wgblas's JavaScript API (index.mjs): ``init``,
 ``cleanup``, ``gpuName``, ``getDevice``, ``getAdapter``, ``sgemm``, ``dgemm``, the gemmtr family (``sgemmtr``,
 ``dgemmtr``, ``ssyrk``, ``dsyrk``, ``ssyr2k``, ``dsyr2k``), ``ssymm``/``dsymm``,
 ``strmm``/``dtrmm``, ``strsm``, ``sgemv``/``dgemv``, ``GpuMatrix``,
-``GpuVector``, ``randomFloat32Array`` and ``randomFloat64Array``. Compute runs in the CUDA
+``GpuVector``, ``randomFloat32Array`` and ``randomFloat64Array``. Beside them stand the
+products of language-model layers, which the reference does not have: ``gemmGrouped`` and
+``gemmGroupedInner`` (16-bit, rows grouped by expert), ``mxQuantize``, ``mxDequantize``,
+``mxGemm`` and ``mxGemmGrouped`` (4-bit floating point), on ``GpuArray`` and ``GpuMxMatrix``
+or another library's CUDA tensors. Compute runs in the CUDA
 library libwgblas_b200.so (include/wgblas.h) with hand-written sm_100a
 kernels; importing the package without that library raises ImportError.
 """

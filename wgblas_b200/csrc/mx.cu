@@ -172,8 +172,9 @@ constexpr int ROWS_AT_ONCE = 4;  // a warp's loads in flight
 // One CTA per two scale tiles: a warp takes whole 256-column lines, eight
 // elements a thread, four threads a block. Bound by memory: 16-byte loads, four
 // in flight a thread; a line's codes are one 128-byte store, the scales are
-// gathered in shared memory and written as one piece. 8192 x 8192 bf16: see the
-// figures at launch_quant.
+// gathered in shared memory and written as one piece. 8192 x 8192 bf16: 31 us, 5.5
+// TB/s of reads and writes (a copy's rate here is 6.55); back, 34 us. Sixteen threads a
+// line and one line in flight a thread took 54 and 65 us.
 template <class T>
 __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
   __shared__ __align__(16) uint8_t sf[1024];
@@ -834,15 +835,15 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
 }
 
 // The form with the least modelled time, as for the 16-bit products (grouped.cu);
-// joining parts costs about 2400 clocks, a pair's start and single accumulator
-// 3500. us in a CUDA graph, operands in L2, m x n x k (groups):
+// joining parts costs about 2700 clocks, a pair's start and single accumulator
+// 3500. us in a CUDA graph, operands in L2, m x n x k (groups), the chosen form's starred:
 //                            pair  128 columns  32 columns  ... split 2  split 4
-//   1024 x 4096 x 4096 (1)   12.2     13.0         -            -         -
-//   128 x 8192 x 4096 (1)    10.0      8.1         -            -         -
-//   1500 x 2048 x 4096 (32)  30.9     29.8         -            -         -
-//   16 x 8192 x 4096 (1)      7.4      6.6         6.3          6.7      11.8
-//   16 x 2048 x 8192 (1)     10.8      9.4         9.2          7.7       6.6
-//   30 x 2048 x 2048 (16)     9.8      9.3         7.8         12.1      33.2
+//   1024 x 4096 x 4096 (1)   12.0*    12.8         -            -         -
+//   128 x 8192 x 4096 (1)     9.8      8.1*        -            -         -
+//   1500 x 2048 x 4096 (32)  30.9     29.8*        -            -         -
+//   16 x 8192 x 4096 (1)      7.3      6.6        6.2*         6.4      11.0
+//   16 x 2048 x 8192 (1)     10.6      9.4        9.2          7.2       6.0*
+//   30 x 2048 x 2048 (16)     9.9      9.2        7.9*         9.8      24.2
 // (a split of 128-column tiles won nowhere by more than 4 % and is not built).
 // A 32-column form needs every group to fit it, which only the number of all rows can show here.
 enum Form { PAIR_256, ONE_128, ONE_32, SPLIT_32_2, SPLIT_32_4, FORMS };
@@ -862,7 +863,7 @@ Form choose(const wg_device *d, const Args &a) {
     const int64_t box = std::min<int64_t>(f.bn, 64), lines = (nv / f.cg + box - 1) / box * box;
     const double block = std::max({nv * 2.0, ((BL + lines) * 128 + 2048) / 65.0, 300.0});
     const double tail = (double)BL * nv * (a.out.type == WG_TYPE_F32 ? 4 : 2) / 20 +
-                        (f.p > 1 ? 2400 : f.cg > 1 ? 3500 : 0);
+                        (f.p > 1 ? 2700 : f.cg > 1 ? 3500 : 0);
     const double t = rounds * (double)((kt + f.p - 1) / f.p) * block + tail;
     if (t < least) {
       least = t;
