@@ -103,6 +103,31 @@ def test_quantize_extremes(wg, device):
     q.destroy()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,cols", [(31, 1000), (333, 777), (1000, 1000), (7205, 2056)])
+def test_quantize_there_and_back(wg, device, dtype, rows, cols):
+    """Quarters of tile pairs and whole ones, rows of whole 16-byte units and others, in both directions."""
+    rng = np.random.default_rng(rows + cols)
+    x = (rng.standard_normal((rows, cols)) * np.exp2(rng.integers(-8, 8, (rows, 1)))).astype(np.float32)
+    for pad in (0, 8, 3):
+        q, x64 = quantized(wg, device, x, dtype, ld=cols + pad)
+        if pad == 0:
+            code, scale = mc.quantize(x64)
+            want_codes, want_scales = mc.pack_codes(code), mc.tile_scales(scale)
+            want = mc.values(code, scale, cols)
+            assert (want == want.astype(np.float32)).all()
+        assert np.array_equal(q.codes.read().reshape(rows, -1), want_codes)
+        assert np.array_equal(q.scales.read(), want_scales)
+        blank = up(wg, np.full(rows * (cols + pad), 7, np.float32), dtype)[0]
+        out = wg.GpuArray.from_(device, blank, dtype)
+        wg.mxDequantize(device, q, out, cols + pad)
+        got = values(wg, out).reshape(rows, cols + pad)
+        # (4-bit elements times a power of two in range: exact in every type)
+        assert np.array_equal(got[:, :cols], want) and (got[:, cols:] == 7).all()
+        out.destroy()
+        q.destroy()
+
+
 @pytest.mark.parametrize("sizes,first,after", [([5, 0, 130, 1], 0, 0), ([128, 128], 0, 3), ([0, 300], 4, 2), ([0], 2, 0)])
 def test_quantize_grouped_rows(wg, device, sizes, first, after):
     rng = np.random.default_rng(9)

@@ -100,6 +100,41 @@ __device__ __forceinline__ uint32_t top_of(const Eight<T> &w) {
   return __float_as_uint(to_float(*reinterpret_cast<const T *>(&h)));
 }
 
+// Eight elements at p, of which the first `valid` exist (zeros instead of the
+// others), at any alignment: the 16-byte units that hold them, shifted into place
+// by words and half words. Memory outside [lo, hi) is not read.
+template <class T>
+__device__ __forceinline__ void load_eight(Eight<T> &out, const T *p, int valid, const T *lo, const T *hi) {
+  constexpr int U = sizeof(T) / 2 + 1, WORDS = 4 * (U - 1);
+  const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15;
+  const T *base = p - off / sizeof(T);
+  if (valid > 0 && base >= lo && base + U * 16 / sizeof(T) <= hi) {
+    uint32_t w[4 * U];
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(base) + i);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+    if (off & 4)
+#pragma unroll
+      for (int i = 0; i < WORDS + 3; i++) w[i] = w[i + 1];
+    if (off & 8)
+#pragma unroll
+      for (int i = 0; i < WORDS + 1; i++) w[i] = w[i + 2];
+    uint32_t x[WORDS];
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) x[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (off & 2) * 8) : w[i];
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; i++) out.w[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i >= valid) out.v[i] = T(0.0f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) out.v[i] = i < valid ? p[i] : T(0.0f);
+  }
+}
+
 // The rows of one scale tile: first row, how many, and its matrix (batch).
 struct TileRows {
   int r0, n, b;
@@ -167,21 +202,35 @@ __device__ __forceinline__ int scale_at(int r, int block) {  // block 0 .. 7 of 
   return (block >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (block & 3);
 }
 
+// A CTA's part of the matrix: two neighbouring scale tiles, of whose rows it takes
+// all (STEP 8: its warps take one line in eight), or a quarter (STEP 32: a warp takes
+// lines r0 + warp, 32 apart, four in all, whose scales are neighbours too).
+struct Part {
+  int tile, tc, r0;
+};
+template <int STEP>
+__device__ __forceinline__ Part part_of(const QuantArgs &a) {
+  const unsigned pairs = (unsigned)(a.tiles_c + 1) >> 1, x = STEP == 32 ? blockIdx.x >> 2 : blockIdx.x;
+  return {(int)(x / pairs), (int)(x % pairs) * 2, STEP == 32 ? (int)(blockIdx.x & 3) * 8 : 0};
+}
+// Elements from a matrix's first to its last (stored rows x cols).
+__device__ __forceinline__ int64_t used_elements(const QuantArgs &a) { return (int64_t)(a.rows - 1) * a.ldx + a.cols; }
+
 constexpr int ROWS_AT_ONCE = 4;  // a warp's loads in flight
 
-// One CTA per two scale tiles: a warp takes whole 256-column lines, eight
+// A CTA per part (launch_rows): a warp takes whole 256-column lines, eight
 // elements a thread, four threads a block. Bound by memory: 16-byte loads, four
 // in flight a thread; a line's codes are one 128-byte store, the scales are
 // gathered in shared memory and written as one piece. 8192 x 8192 bf16: 31 us, 5.5
 // TB/s of reads and writes (a copy's rate here is 6.55); back, 34 us. Sixteen threads a
 // line and one line in flight a thread took 54 and 65 us.
-template <class T>
+template <class T, int STEP>
 __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
   __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
-  const int pairs = (a.tiles_c + 1) >> 1;
-  const int tile = (int)(blockIdx.x / (unsigned)pairs), tc = (int)(blockIdx.x % (unsigned)pairs) * 2;
+  const Part part = part_of<STEP>(a);
+  const int tile = part.tile, tc = part.tc;
   const TileRows t = rows_of_tile(a, tile);
   if (t.n <= 0) return;
   reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = 0;
@@ -193,10 +242,12 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
   // (the whole warp takes one way: the lines' shuffles need all its lanes)
   const bool wide = __all_sync(0xffffffffu, valid >= 8 && ((uintptr_t)X & 15) == 0 && a.ldx * sizeof(T) % 16 == 0);
   uint8_t *codes = a.codes + (int64_t)t.b * a.rows * a.pitch + col / 2;
-  const T *src = X + (t.r0 + (int64_t)warp) * a.ldx;
-  uint8_t *dst = codes + (t.r0 + (int64_t)warp) * a.pitch;
+  int r = part.r0 + warp;
+  const T *src = X + (t.r0 + (int64_t)r) * a.ldx;
+  uint8_t *dst = codes + (t.r0 + (int64_t)r) * a.pitch;
+  const T *lo = static_cast<const T *>(a.X) + t.b * a.strideX, *hi = lo + used_elements(a);
   uint8_t *sfb = sf + (c >> 4) * 512 + (c >> 2 & 3);
-  const int64_t src_step = 8 * a.ldx, dst_step = 8 * a.pitch;
+  const int64_t src_step = STEP * a.ldx, dst_step = STEP * a.pitch;
   // Rounds one line's eight elements; `r` is the line within the tile.
   auto round = [&](const Eight<T> &w, uint8_t *to, int r) {
     uint32_t top = top_of(w);
@@ -217,7 +268,7 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
   auto batch = [&](auto count, int r, const T *from, uint8_t *to) {
     constexpr int N = decltype(count)::value;
     Eight<T> w[N];
-    const int last = (t.n - 1 - r) >> 3;
+    const int last = (t.n - 1 - r) / STEP;
 #pragma unroll
     for (int u = 0; u < N; u++) {
       const T *p = from + min(u, last) * src_step;
@@ -225,38 +276,46 @@ __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
       } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[u].v[i] = i < valid ? p[i] : T(0.0f);
+        load_eight(w[u], p, valid, lo, hi);
       }
     }
 #pragma unroll
     for (int u = 0; u < N; u++)
-      if (u <= last) round(w[u], to + u * dst_step, r + 8 * u);
+      if (u <= last) round(w[u], to + u * dst_step, r + STEP * u);
   };
-  int r = warp;
-  if (wide && t.n > 64)
-    for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
-      Eight<T> w[ROWS_AT_ONCE];
+  if constexpr (STEP == 32) {
+    if (r < t.n) batch(std::integral_constant<int, 4>(), r, src, dst);
+  } else {
+    if (wide && t.n > 64)
+      for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
+        Eight<T> w[ROWS_AT_ONCE];
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step)
+        for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step)
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+          for (int i = 0; i < (int)sizeof(T) / 2; i++) w[u].w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) round(w[u], dst, r + 8 * u);
-    }
-  // The rest (all of a short tile, at once), and lines that wide loads cannot read.
-  constexpr int REST = sizeof(T) == 2 ? 8 : 4;
-  for (; r < t.n; r += 8 * REST, src += REST * src_step, dst += REST * dst_step)
-    batch(std::integral_constant<int, REST>(), r, src, dst);
+        for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) round(w[u], dst, r + 8 * u);
+      }
+    // The rest (all of a short tile, at once), and lines that wide loads cannot read.
+    constexpr int REST = 8;
+    for (; r < t.n; r += 8 * REST, src += REST * src_step, dst += REST * dst_step)
+      batch(std::integral_constant<int, REST>(), r, src, dst);
+  }
   __syncthreads();
   // (the second tile exists unless the tile row has an odd number of them)
-  if (threadIdx.x < 128 || tc + 1 < a.tiles_c) tile_scales(a, tile, tc)[threadIdx.x] = reinterpret_cast<const uint32_t *>(sf)[threadIdx.x];
+  constexpr int WORDS = STEP == 32 ? 32 : 128;
+  if (threadIdx.x < WORDS || (threadIdx.x < 2 * WORDS && tc + 1 < a.tiles_c)) {
+    const int i = (int)(threadIdx.x / WORDS) * 128 + part.r0 * 4 + (int)(threadIdx.x % WORDS);
+    tile_scales(a, tile, tc)[i] = reinterpret_cast<const uint32_t *>(sf)[i];
+  }
 }
 
 // The transposed form: X holds the matrix's columns as its rows. One CTA per
 // scale tile; a thread takes two neighbouring rows of the result and one block
 // of them, 32 of X's lines: its loads are independent, and a warp's are 64
-// neighbouring elements.
+// neighbouring elements. The codes go through shared memory, so that a row's four
+// blocks are stored together (8192 x 8192 bf16: 34.5 us, with each thread's 16 bytes
+// stored on their own 38.2).
 template <class T>
 struct Two {
   T v[2];
@@ -264,6 +323,7 @@ struct Two {
 template <class T>
 __global__ void __launch_bounds__(256) mx_quantize_t(const QuantArgs a) {
   __shared__ __align__(16) uint8_t sf[512];
+  __shared__ uint4 out[128 * 5];  // the tile's codes, four blocks a row (and one for the banks)
   wg_pdl_wait();
   wg_pdl_trigger();
   const int tile = (int)(blockIdx.x / (unsigned)a.tiles_c), tc = (int)(blockIdx.x % (unsigned)a.tiles_c);
@@ -310,13 +370,18 @@ __global__ void __launch_bounds__(256) mx_quantize_t(const QuantArgs a) {
         code[i] = encode8(y);
       }
       if (p == 0 || both) {
-        const int64_t at = ((int64_t)t.b * a.rows + t.r0 + r + p) * a.pitch + col / 2;
-        *reinterpret_cast<uint4 *>(a.codes + at) = make_uint4(code[0], code[1], code[2], code[3]);
+        out[(r + p) * 5 + blk] = make_uint4(code[0], code[1], code[2], code[3]);
         sf[scale_at(r + p, blk)] = (uint8_t)e;
       }
     }
   }
   __syncthreads();
+  for (int i = threadIdx.x; i < t.n * 4; i += 256) {
+    const int row = i >> 2, b = i & 3;
+    const int64_t at = tc * 64 + b * 16;
+    if (at < a.pitch)
+      *reinterpret_cast<uint4 *>(a.codes + ((int64_t)t.b * a.rows + t.r0 + row) * a.pitch + at) = out[row * 5 + b];
+  }
   if (threadIdx.x < 128) tile_scales(a, tile, tc)[threadIdx.x] = reinterpret_cast<const uint32_t *>(sf)[threadIdx.x];
 }
 
@@ -345,31 +410,33 @@ __device__ __forceinline__ void decode4(uint32_t code, float scale, float *y) {
   }
 }
 
-// X here is the output (rows x cols, ldx). The quantiser's division of the work;
-// a thread's store is 16 bytes, a warp's 512 neighbouring ones (an fp32 line
+// X here is the output (rows x cols, ldx), of rows of whole 16-byte units. The
+// quantiser's division of the work; a thread's store is 16 bytes, a warp's 512 neighbouring ones (an fp32 line
 // takes two).
-template <class T>
+template <class T, int STEP>
 __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
   constexpr int E = 16 / sizeof(T), PASSES = 8 / E;
   __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
-  const int pairs = (a.tiles_c + 1) >> 1;
-  const int tile = (int)(blockIdx.x / (unsigned)pairs), tc = (int)(blockIdx.x % (unsigned)pairs) * 2;
+  const Part part = part_of<STEP>(a);
+  const int tile = part.tile, tc = part.tc;
   const TileRows t = rows_of_tile(a, tile);
   if (t.n <= 0) return;
   if (threadIdx.x < 128 || tc + 1 < a.tiles_c) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = tile_scales(a, tile, tc)[threadIdx.x];
   __syncthreads();
-  const int warp = threadIdx.x >> 5, c = threadIdx.x & 31;
+  const int c = threadIdx.x & 31, first = part.r0 + (int)(threadIdx.x >> 5);
+  T *X = static_cast<T *>(const_cast<void *>(a.X)) + t.b * a.strideX;
+  const uint8_t *codes = a.codes + (int64_t)t.b * a.rows * a.pitch;
 #pragma unroll
   for (int p = 0; p < PASSES; p++) {
     const int in_tiles = p * 32 * E + c * E, col = tc * 128 + in_tiles;
     if (col >= a.cols) return;
-    const uint8_t *src = a.codes + ((int64_t)t.b * a.rows + t.r0 + warp) * a.pitch + col / 2;
-    T *dst = static_cast<T *>(const_cast<void *>(a.X)) + t.b * a.strideX + (t.r0 + (int64_t)warp) * a.ldx + col;
+    const uint8_t *src = codes + (t.r0 + (int64_t)first) * a.pitch + col / 2;
+    T *dst = X + (t.r0 + (int64_t)first) * a.ldx + col;
     const uint8_t *sfb = sf + scale_at(0, in_tiles >> 5);
-    const int64_t src_step = 8 * a.pitch, dst_step = 8 * a.ldx;
-    const bool wide = col + E <= a.cols && ((uintptr_t)dst & 15) == 0 && a.ldx * sizeof(T) % 16 == 0;
+    const int64_t src_step = STEP * a.pitch, dst_step = STEP * a.ldx;
+    const bool wide = col + E <= a.cols;
     auto load = [&](const uint8_t *at) -> uint32_t {
       if constexpr (E == 8) return __ldg(reinterpret_cast<const uint32_t *>(at));
       else return __ldg(reinterpret_cast<const uint16_t *>(at));
@@ -390,22 +457,59 @@ __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
           if (col + i < a.cols) to[i] = y[i];
       }
     };
-    int r = warp;
-    for (; r + 8 * (ROWS_AT_ONCE - 1) < t.n; r += 8 * ROWS_AT_ONCE) {
+    int r = first;
+    for (; r + STEP * (ROWS_AT_ONCE - 1) < t.n; r += STEP * ROWS_AT_ONCE) {
       uint32_t code[ROWS_AT_ONCE];
 #pragma unroll
       for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step) code[u] = load(src);
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) store(code[u], dst, r + 8 * u);
+      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) store(code[u], dst, r + STEP * u);
     }
     if (r < t.n) {
-      const int last = (t.n - 1 - r) >> 3;
+      const int last = (t.n - 1 - r) / STEP;
       uint32_t code[ROWS_AT_ONCE];
 #pragma unroll
       for (int u = 0; u < ROWS_AT_ONCE; u++) code[u] = load(src + min(u, last) * src_step);
 #pragma unroll
       for (int u = 0; u < ROWS_AT_ONCE; u++)
-        if (u <= last) store(code[u], dst + u * dst_step, r + 8 * u);
+        if (u <= last) store(code[u], dst + u * dst_step, r + STEP * u);
+    }
+  }
+}
+
+// Rows of any alignment: lane c stores elements c, c + 32, ... of a line, so that a
+// warp's store is 32 neighbouring ones; their codes are in words of other lanes.
+// (16-byte-aligned threads storing element by element: 8001 x 8001 bf16 183 us, this 63.)
+template <class T>
+__global__ void __launch_bounds__(256) mx_dequantize_unaligned(const QuantArgs a) {
+  __shared__ __align__(16) uint8_t sf[1024];
+  wg_pdl_wait();
+  wg_pdl_trigger();
+  const Part part = part_of<32>(a);
+  const int tile = part.tile, tc = part.tc;
+  const TileRows t = rows_of_tile(a, tile);
+  if (t.n <= 0) return;
+  if (threadIdx.x < 128 || tc + 1 < a.tiles_c) reinterpret_cast<uint32_t *>(sf)[threadIdx.x] = tile_scales(a, tile, tc)[threadIdx.x];
+  __syncthreads();
+  const int c = threadIdx.x & 31, first = part.r0 + (int)(threadIdx.x >> 5);
+  T *X = static_cast<T *>(const_cast<void *>(a.X)) + t.b * a.strideX;
+  const uint8_t *codes = a.codes + (int64_t)t.b * a.rows * a.pitch;
+  const bool in = tc * 128 + c * 8 < ((a.cols + 31) & ~31);  // this lane's word of codes exists
+  uint32_t word[4];
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int r = first + 32 * u;
+    word[u] = in && r < t.n ? __ldg(reinterpret_cast<const uint32_t *>(codes + (t.r0 + (int64_t)r) * a.pitch) + tc * 16 + c) : 0;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int r = first + 32 * u;
+    T *to = X + (t.r0 + (int64_t)r) * a.ldx + tc * 128 + c;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float f[4];
+      decode4(__shfl_sync(0xffffffffu, word[u], 4 * i + (c >> 3)) >> (4 * (c & 7)) & 15u, scale_value(sf[scale_at(r, i)]), f);
+      if (r < t.n && tc * 128 + i * 32 + c < a.cols) to[i * 32] = from_float<T>(f[0]);
     }
   }
 }
@@ -774,13 +878,36 @@ wg_status check_quant(const wg_device *d, int type, int64_t batch, int64_t rows,
   return groups > 0 ? wgg::check_offsets(offsets) : WG_OK;
 }
 
-wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const QuantArgs), const QuantArgs &a, int ctas_a_row) {
-  const int64_t tiles = a.offsets ? tiles_of(a.rows) + a.groups : (int64_t)a.batch * a.tiles_r;
-  if (tiles * ctas_a_row >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
+wg_status launch_quant(wg_device *d, const char *family, void (*kern)(const QuantArgs), const QuantArgs &a, int64_t ctas) {
+  if (ctas >= LIM) return wg_fail(WG_ERR_INVALID_ARGUMENT, "too many elements for one call");
   wg_launch_scope scope(d, family);
-  WG_CUDA(wg_launch_pdl(kern, dim3((unsigned)(tiles * ctas_a_row)), dim3(256), 0, d->stream, a));
+  WG_CUDA(wg_launch_pdl(kern, dim3((unsigned)ctas), dim3(256), 0, d->stream, a));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
+}
+int64_t row_tiles(const QuantArgs &a) { return a.offsets ? tiles_of(a.rows) + a.groups : (int64_t)a.batch * a.tiles_r; }
+
+// The row forms: CTAs of quarters of a tile pair, of whole ones for 16-bit matrices
+// of whole 16-byte units with at least three pairs an SM. us, whole against quarters,
+// bf16: 1000 x 1024 4.3 / 2.4 (back 4.4 / 2.4), 2048 x 4096 7.6 / 7.1, 4096 x 4096
+// 10.1 / 11.3, 8192 x 8192 32.0 / 37.8 (back 33.8 / 39.3), unaligned 4000 x 4001 20.5 /
+// 17.4; fp32: 4096 x 4096 14.1 / 13.9, 8192 x 8192 47.2 / 45.6 (back 55.7 / 49.8).
+template <class T>
+wg_status launch_rows(wg_device *d, const char *family, bool back, const QuantArgs &a) {
+  const int64_t pairs = row_tiles(a) * ((a.tiles_c + 1) / 2);
+  const bool aligned = (((uintptr_t)a.X | (uintptr_t)a.ldx * sizeof(T) |
+                         (a.batch > 1 ? (uintptr_t)a.strideX * sizeof(T) : 0)) & 15) == 0;
+  if constexpr (sizeof(T) == 2)
+    if (aligned && pairs >= (int64_t)3 * d->sm_count)
+      return launch_quant(d, family, back ? mx_dequantize<T, 8> : mx_quantize<T, 8>, a, pairs);
+  return launch_quant(d, family, !back     ? mx_quantize<T, 32>
+                                 : aligned ? mx_dequantize<T, 32>
+                                           : mx_dequantize_unaligned<T>, a, pairs * 4);
+}
+wg_status launch_rows_of(wg_device *d, const char *family, bool back, const QuantArgs &a) {
+  return a.xtype == WG_TYPE_F32    ? launch_rows<float>(d, family, back, a)
+         : a.xtype == WG_TYPE_BF16 ? launch_rows<__nv_bfloat16>(d, family, back, a)
+                                   : launch_rows<__half>(d, family, back, a);
 }
 
 bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *ptr, int rank, const cuuint64_t *dims,
@@ -947,12 +1074,10 @@ extern "C" wg_status wg_mx_quantize_dev(wg_device *d, int type, int trans, int64
                  static_cast<uint8_t *>(scales), pitch_of(cols), (int)tiles_of(rows), (int)tiles_of(cols), (int)batch,
                  groups ? offsets : nullptr, (int)groups, d->dwords};
   return wg_timed(d, gpu_ms, [&] {
-    void (*kern)(const QuantArgs);
-    if (trans)
-      kern = type == WG_TYPE_F32 ? mx_quantize_t<float> : type == WG_TYPE_BF16 ? mx_quantize_t<__nv_bfloat16> : mx_quantize_t<__half>;
-    else
-      kern = type == WG_TYPE_F32 ? mx_quantize<float> : type == WG_TYPE_BF16 ? mx_quantize<__nv_bfloat16> : mx_quantize<__half>;
-    return launch_quant(d, "mx_quantize", kern, a, trans ? a.tiles_c : (a.tiles_c + 1) / 2);
+    if (!trans) return launch_rows_of(d, "mx_quantize", false, a);
+    return launch_quant(d, "mx_quantize", type == WG_TYPE_F32    ? mx_quantize_t<float>
+                                          : type == WG_TYPE_BF16 ? mx_quantize_t<__nv_bfloat16>
+                                                                 : mx_quantize_t<__half>, a, row_tiles(a) * a.tiles_c);
   });
 }
 
@@ -977,12 +1102,7 @@ extern "C" wg_status wg_mx_dequantize_dev(wg_device *d, int type, int64_t batch,
   QuantArgs a = {X, ldx, strideX, type, (int)rows, (int)cols, static_cast<uint8_t *>(const_cast<void *>(codes)),
                  static_cast<uint8_t *>(const_cast<void *>(scales)), pitch_of(cols), (int)tiles_of(rows),
                  (int)tiles_of(cols), (int)batch, groups ? offsets : nullptr, (int)groups, d->dwords};
-  return wg_timed(d, gpu_ms, [&] {
-    return launch_quant(d, "mx_dequantize",
-                        type == WG_TYPE_F32 ? mx_dequantize<float>
-                        : type == WG_TYPE_BF16 ? mx_dequantize<__nv_bfloat16> : mx_dequantize<__half>, a,
-                        (a.tiles_c + 1) / 2);
-  });
+  return wg_timed(d, gpu_ms, [&] { return launch_rows_of(d, "mx_dequantize", true, a); });
 }
 
 extern "C" wg_status wg_mx_gemm_dev(wg_device *d, int ctype, int64_t m, int64_t n, int64_t k, float alpha,
