@@ -99,6 +99,31 @@ def test_strided_views(wg, dev):
                        torch.empty((m + 2, n), device="cuda"), n)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3, 5, 7])
+@pytest.mark.parametrize("rows,cols", [(1, 5), (3, 40), (70, 301), (129, 520)])
+def test_quantize_alignment_of_the_bases(wg, dev, dtype, shift, rows, cols):
+    """A matrix anywhere in memory gives the codes of its aligned copy, and back, and its neighbours stay."""
+    flat = torch.full((shift + rows * cols + 9,), float("nan"), device="cuda", dtype=dtype)
+    x = flat[shift:shift + rows * cols].view(rows, cols)
+    x.copy_(torch.randn(rows, cols, device="cuda"))
+    pitch = -(-cols // 8) * 8
+    copy = torch.zeros((rows, pitch), device="cuda", dtype=dtype)
+    copy[:, :cols] = x
+    for trans in (N, T):
+        r, c = (cols, rows) if trans == T else (rows, cols)
+        q, want = wg.GpuMxMatrix.empty(dev, r, c), wg.GpuMxMatrix.empty(dev, r, c)
+        wg.mxQuantize(dev, trans, r, c, x, cols, q)
+        wg.mxQuantize(dev, trans, r, c, copy, pitch, want)
+        assert (q.codes.read() == want.codes.read()).all() and (q.scales.read() == want.scales.read()).all()
+        out = torch.full((shift + r * c + 9,), 7.0, device="cuda", dtype=dtype)
+        wg.mxDequantize(dev, q, out[shift:], c)
+        back = out[shift:shift + r * c].double().cpu().numpy().reshape(r, c)
+        assert (back == wg.mxDecode(q.codes.read(), q.scales.read(), r, c)).all()
+        assert (out[:shift] == 7).all() and (out[shift + r * c:] == 7).all()
+        q.destroy(), want.destroy()
+
+
 def test_a_host_tensor_is_refused(wg, dev):
     x, w, off = make([4], 8, 8)
     with pytest.raises(wg.Error, match="A must be a GpuArray or a CUDA tensor."):
