@@ -19,9 +19,12 @@
 /* Set once by setup(): the classes, and the type names of foreign dtype objects. */
 static PyObject *t_device, *t_array, *t_mx, *foreign;
 /* Interned attribute and method names. */
-static PyObject *n_handle, *n_value, *n_benchmark, *n_ordinal, *n_device, *n_ptr, *n_length, *n_dtype, *n_is_cuda,
-    *n_data_ptr, *n_get_device, *n_is_contiguous, *n_numel, *n_rows, *n_cols, *n_batch, *n_groups, *n_codes, *n_scales,
-    *n_pcodes, *n_pscales;
+static PyObject *n_handle, *n_value, *n_benchmark, *n_ordinal, *n_dtype, *n_is_cuda, *n_data_ptr, *n_get_device,
+    *n_is_contiguous, *n_numel;
+/* Where GpuArray and GpuMxMatrix objects keep their __slots__ (asked of the classes by
+ * setup(): an attribute lookup for each of a matrix's nine costs 0.3 microseconds). */
+static Py_ssize_t a_device, a_ptr, a_length, a_dtype, m_device, m_rows, m_cols, m_batch, m_groups, m_codes, m_scales,
+    m_pcodes, m_pscales;
 
 enum { T_F32 = WG_TYPE_F32, T_BF16 = WG_TYPE_BF16, T_F16 = WG_TYPE_F16, T_I32 = 3, T_U8 = 4 };
 static const int item_bytes[] = {4, 2, 2, 4, 1};
@@ -55,17 +58,24 @@ static int attr_i64(PyObject *x, PyObject *name, int64_t *out) {
   return ok;
 }
 
+static int get_ptr(PyObject *v, uintptr_t *out) {
+  if (!v || !PyLong_CheckExact(v)) return 0;
+  *out = (uintptr_t)PyLong_AsUnsignedLongLong(v);
+  if (*out != (uintptr_t)-1 || !PyErr_Occurred()) return 1;
+  PyErr_Clear();
+  return 0;
+}
+
 static int attr_ptr(PyObject *x, PyObject *name, uintptr_t *out) {
   PyObject *v = PyObject_GetAttr(x, name);
-  int ok = v && PyLong_CheckExact(v);
-  if (ok) {
-    *out = (uintptr_t)PyLong_AsUnsignedLongLong(v);
-    if (PyErr_Occurred()) ok = 0;
-  }
+  int ok = get_ptr(v, out);
   Py_XDECREF(v);
   PyErr_Clear();
   return ok;
 }
+
+/* A slot's object (borrowed; NULL when it was never set). */
+static PyObject *slot(PyObject *x, Py_ssize_t at) { return *(PyObject **)((char *)x + at); }
 
 static int call_i64(PyObject *x, PyObject *method, int64_t *out) {
   PyObject *v = PyObject_CallMethodNoArgs(x, method);
@@ -128,13 +138,9 @@ static int get_device(PyObject *x, device *out) {
 
 static int get_operand(const device *d, PyObject *x, operand *out) {
   if ((PyObject *)Py_TYPE(x) == t_array) {
-    PyObject *dev = PyObject_GetAttr(x, n_device), *type = PyObject_GetAttr(x, n_dtype);
-    int ok = dev == d->obj;
-    out->type = type_of(type);
-    Py_XDECREF(dev);
-    Py_XDECREF(type);
-    PyErr_Clear();
-    return ok && out->type >= 0 && attr_ptr(x, n_ptr, &out->p) && out->p && attr_i64(x, n_length, &out->n);
+    out->type = type_of(slot(x, a_dtype));
+    return slot(x, a_device) == d->obj && out->type >= 0 && get_ptr(slot(x, a_ptr), &out->p) && out->p &&
+           get_i64(slot(x, a_length), &out->n);
   }
   if (!is_true(PyObject_GetAttr(x, n_is_cuda))) return 0;
   PyObject *dtype = PyObject_GetAttr(x, n_dtype);
@@ -157,29 +163,16 @@ typedef struct {
   uintptr_t codes, scales;
 } mx;
 
-static int live(PyObject *x) { /* steals x: a GpuArray that was not destroyed, or another's tensor */
-  int ok = x != NULL;
-  if (ok && (PyObject *)Py_TYPE(x) == t_array) {
-    uintptr_t p = 0;
-    ok = attr_ptr(x, n_ptr, &p) && p;
-  }
-  Py_XDECREF(x);
-  PyErr_Clear();
-  return ok;
+static int live(PyObject *x) { /* a GpuArray that was not destroyed, or another's tensor */
+  uintptr_t p = 0;
+  return x && ((PyObject *)Py_TYPE(x) != t_array || (get_ptr(slot(x, a_ptr), &p) && p));
 }
 
 static int get_mx(const device *d, PyObject *x, mx *out) {
-  if ((PyObject *)Py_TYPE(x) != t_mx) return 0;
-  PyObject *dev = PyObject_GetAttr(x, n_device);
-  Py_XDECREF(dev);
-  if (dev != d->obj) {
-    PyErr_Clear();
-    return 0;
-  }
-  return attr_i64(x, n_rows, &out->rows) && attr_i64(x, n_cols, &out->cols) && attr_i64(x, n_batch, &out->batch) &&
-         attr_i64(x, n_groups, &out->groups) && attr_ptr(x, n_pcodes, &out->codes) &&
-         attr_ptr(x, n_pscales, &out->scales) && live(PyObject_GetAttr(x, n_codes)) &&
-         live(PyObject_GetAttr(x, n_scales));
+  return (PyObject *)Py_TYPE(x) == t_mx && slot(x, m_device) == d->obj && get_i64(slot(x, m_rows), &out->rows) &&
+         get_i64(slot(x, m_cols), &out->cols) && get_i64(slot(x, m_batch), &out->batch) &&
+         get_i64(slot(x, m_groups), &out->groups) && get_ptr(slot(x, m_pcodes), &out->codes) &&
+         get_ptr(slot(x, m_pscales), &out->scales) && live(slot(x, m_codes)) && live(slot(x, m_scales));
 }
 
 /* ---- sizes ------------------------------------------------------------------ */
@@ -417,18 +410,31 @@ static PyObject *mx_wrap(PyObject *self, PyObject *const *v, Py_ssize_t nv) {
   PyObject *x = t->tp_alloc(t, 0);
   if (!x) return NULL;
   PyObject *pc = PyLong_FromUnsignedLongLong(c.p), *ps = PyLong_FromUnsignedLongLong(s.p);
-  int bad = !pc || !ps || PyObject_SetAttr(x, n_device, v[0]) || PyObject_SetAttr(x, n_codes, v[1]) ||
-            PyObject_SetAttr(x, n_scales, v[2]) || PyObject_SetAttr(x, n_rows, v[3]) ||
-            PyObject_SetAttr(x, n_cols, v[4]) || PyObject_SetAttr(x, n_batch, v[5]) ||
-            PyObject_SetAttr(x, n_groups, v[6]) || PyObject_SetAttr(x, n_pcodes, pc) ||
-            PyObject_SetAttr(x, n_pscales, ps);
-  Py_XDECREF(pc);
-  Py_XDECREF(ps);
-  if (bad) {
+  if (!pc || !ps) {
+    Py_XDECREF(pc);
+    Py_XDECREF(ps);
     Py_DECREF(x);
     return NULL;
   }
+  PyObject *const value[] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], pc, ps};
+  const Py_ssize_t at[] = {m_device, m_codes, m_scales, m_rows, m_cols, m_batch, m_groups, m_pcodes, m_pscales};
+  for (int i = 0; i < 9; i++) {
+    if (i < 7) Py_INCREF(value[i]); /* (pc and ps are new) */
+    *(PyObject **)((char *)x + at[i]) = value[i];
+  }
   return x;
+}
+
+/* Where the class keeps its slot `name`; -1 with an exception set. */
+static Py_ssize_t slot_of(PyObject *type, const char *name) {
+  PyObject *v = PyObject_GetAttrString(type, name);
+  if (!v) return -1;
+  Py_ssize_t at = -1;
+  if (Py_TYPE(v) == &PyMemberDescr_Type && ((PyMemberDescrObject *)v)->d_member->type == Py_T_OBJECT_EX)
+    at = ((PyMemberDescrObject *)v)->d_member->offset;
+  else PyErr_Format(PyExc_TypeError, "%s is not a slot", name);
+  Py_DECREF(v);
+  return at;
 }
 
 /* setup(Device, GpuArray, GpuMxMatrix, foreign type names) */
@@ -437,6 +443,16 @@ static PyObject *setup(PyObject *self, PyObject *args) {
   PyObject *d, *a, *m, *f;
   if (!PyArg_ParseTuple(args, "O!O!O!O!", &PyType_Type, &d, &PyType_Type, &a, &PyType_Type, &m, &PyDict_Type, &f))
     return NULL;
+  const struct {
+    PyObject *type;
+    Py_ssize_t *at;
+    const char *name;
+  } slots[] = {{a, &a_device, "device"}, {a, &a_ptr, "ptr"}, {a, &a_length, "length"}, {a, &a_dtype, "dtype"},
+               {m, &m_device, "device"}, {m, &m_rows, "rows"}, {m, &m_cols, "cols"}, {m, &m_batch, "batch"},
+               {m, &m_groups, "groups"}, {m, &m_codes, "codes"}, {m, &m_scales, "scales"}, {m, &m_pcodes, "_codes"},
+               {m, &m_pscales, "_scales"}};
+  for (size_t i = 0; i < sizeof slots / sizeof slots[0]; i++)
+    if ((*slots[i].at = slot_of(slots[i].type, slots[i].name)) < 0) return NULL;
   Py_INCREF(d);
   Py_INCREF(a);
   Py_INCREF(m);
@@ -459,11 +475,8 @@ PyMODINIT_FUNC PyInit__fast(void) {
     PyObject **at;
     const char *name;
   } const table[] = {{&n_handle, "_handle"}, {&n_value, "value"}, {&n_benchmark, "benchmark"}, {&n_ordinal, "ordinal"},
-                     {&n_device, "device"}, {&n_ptr, "ptr"}, {&n_length, "length"}, {&n_dtype, "dtype"},
-                     {&n_is_cuda, "is_cuda"}, {&n_data_ptr, "data_ptr"}, {&n_get_device, "get_device"},
-                     {&n_is_contiguous, "is_contiguous"}, {&n_numel, "numel"}, {&n_rows, "rows"}, {&n_cols, "cols"},
-                     {&n_batch, "batch"}, {&n_groups, "groups"}, {&n_codes, "codes"}, {&n_scales, "scales"},
-                     {&n_pcodes, "_codes"}, {&n_pscales, "_scales"}};
+                     {&n_dtype, "dtype"}, {&n_is_cuda, "is_cuda"}, {&n_data_ptr, "data_ptr"},
+                     {&n_get_device, "get_device"}, {&n_is_contiguous, "is_contiguous"}, {&n_numel, "numel"}};
   for (size_t i = 0; i < sizeof table / sizeof table[0]; i++)
     if (!(*table[i].at = PyUnicode_InternFromString(table[i].name))) return NULL;
   return PyModule_Create(&module);
