@@ -221,8 +221,8 @@ constexpr int ROWS_AT_ONCE = 4;  // a warp's loads in flight
 // A CTA per part (launch_rows): a warp takes whole 256-column lines, eight
 // elements a thread, four threads a block. Bound by memory: 16-byte loads, four
 // in flight a thread; a line's codes are one 128-byte store, the scales are
-// gathered in shared memory and written as one piece. 8192 x 8192 bf16: 31 us, 5.5
-// TB/s of reads and writes (a copy's rate here is 6.55); back, 34 us. Sixteen threads a
+// gathered in shared memory and written as one piece. 8192 x 8192 bf16: 32 us, 5.3
+// TB/s of reads and writes (a copy's rate here is 6.55); back, 33 us. Sixteen threads a
 // line and one line in flight a thread took 54 and 65 us.
 template <class T, int STEP>
 __global__ void __launch_bounds__(256) mx_quantize(const QuantArgs a) {
@@ -411,11 +411,12 @@ __device__ __forceinline__ void decode4(uint32_t code, float scale, float *y) {
 }
 
 // X here is the output (rows x cols, ldx), of rows of whole 16-byte units. The
-// quantiser's division of the work; a thread's store is 16 bytes, a warp's 512 neighbouring ones (an fp32 line
-// takes two).
+// quantiser's division of the work; a thread's store is 16 bytes, a warp's 512
+// neighbouring ones (an fp32 line takes two). Whole tile pairs load eight lines of codes
+// at once (4096 x 4096 bf16: 9.1 us, four at once 12.9).
 template <class T, int STEP>
 __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
-  constexpr int E = 16 / sizeof(T), PASSES = 8 / E;
+  constexpr int E = 16 / sizeof(T), PASSES = 8 / E, AT_ONCE = STEP == 8 ? 8 : 4;
   __shared__ __align__(16) uint8_t sf[1024];
   wg_pdl_wait();
   wg_pdl_trigger();
@@ -458,20 +459,20 @@ __global__ void __launch_bounds__(256) mx_dequantize(const QuantArgs a) {
       }
     };
     int r = first;
-    for (; r + STEP * (ROWS_AT_ONCE - 1) < t.n; r += STEP * ROWS_AT_ONCE) {
-      uint32_t code[ROWS_AT_ONCE];
+    for (; r + STEP * (AT_ONCE - 1) < t.n; r += STEP * AT_ONCE) {
+      uint32_t code[AT_ONCE];
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, src += src_step) code[u] = load(src);
+      for (int u = 0; u < AT_ONCE; u++, src += src_step) code[u] = load(src);
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++, dst += dst_step) store(code[u], dst, r + STEP * u);
+      for (int u = 0; u < AT_ONCE; u++, dst += dst_step) store(code[u], dst, r + STEP * u);
     }
     if (r < t.n) {
       const int last = (t.n - 1 - r) / STEP;
-      uint32_t code[ROWS_AT_ONCE];
+      uint32_t code[AT_ONCE];
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++) code[u] = load(src + min(u, last) * src_step);
+      for (int u = 0; u < AT_ONCE; u++) code[u] = load(src + min(u, last) * src_step);
 #pragma unroll
-      for (int u = 0; u < ROWS_AT_ONCE; u++)
+      for (int u = 0; u < AT_ONCE; u++)
         if (u <= last) store(code[u], dst + u * dst_step, r + STEP * u);
     }
   }
@@ -890,7 +891,7 @@ int64_t row_tiles(const QuantArgs &a) { return a.offsets ? tiles_of(a.rows) + a.
 // The row forms: CTAs of quarters of a tile pair, of whole ones for 16-bit matrices
 // of whole 16-byte units with at least three pairs an SM. us, whole against quarters,
 // bf16: 1000 x 1024 4.3 / 2.4 (back 4.4 / 2.4), 2048 x 4096 7.6 / 7.1, 4096 x 4096
-// 10.1 / 11.3, 8192 x 8192 32.0 / 37.8 (back 33.8 / 39.3), unaligned 4000 x 4001 20.5 /
+// 10.1 / 11.3 (back 9.1 / 10.3), 8192 x 8192 32.0 / 37.8 (back 33.1 / 39.3), unaligned 4000 x 4001 20.5 /
 // 17.4; fp32: 4096 x 4096 14.1 / 13.9, 8192 x 8192 47.2 / 45.6 (back 55.7 / 49.8).
 template <class T>
 wg_status launch_rows(wg_device *d, const char *family, bool back, const QuantArgs &a) {
