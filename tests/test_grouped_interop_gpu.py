@@ -99,6 +99,21 @@ def test_strided_views(wg, dev):
                        torch.empty((m + 2, n), device="cuda"), n)
 
 
+@pytest.mark.parametrize("stride,ld", [(8, 64), (64, 64), (3, 70), (0, 64)])
+@pytest.mark.parametrize("trans", [N, T])
+def test_experts_whose_matrices_overlap(wg, dev, trans, stride, ld):
+    """Weights that share memory (windows of one matrix, or one matrix for all) are only read."""
+    sizes, n, k = [40, 0, 90, 7], 48, 64
+    rows, cols = (n, k) if trans == T else (k, n)
+    flat = torch.randn(3 * stride + rows * ld, device="cuda").to(torch.bfloat16)
+    w = torch.stack([flat[g * stride:g * stride + rows * ld].view(rows, ld)[:, :cols] for g in range(4)])
+    x, _, off = make(sizes, n, k)
+    y = torch.zeros((sum(sizes), n), device="cuda")
+    wg.gemmGrouped(dev, trans, 4, sum(sizes), n, k, 1.0, x, k, flat, ld, stride, off, 0.0, y, n)
+    want, mag = rows64(x, w, off, trans == T)
+    check(y, want, mag, k, "float32")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shift", [0, 1, 2, 3, 5, 7])
 @pytest.mark.parametrize("rows,cols", [(1, 5), (3, 40), (70, 301), (129, 520)])
