@@ -85,7 +85,8 @@ wg_status wg_device_props_get(const wg_device *dev, wg_device_props *props);
 /* The stream all of this handle's work is ordered on (a cudaStream_t). */
 wg_status wg_device_stream(const wg_device *dev, void **stream);
 /* Orders this handle's work on a caller-owned cudaStream_t instead; NULL
- * restores the handle's own stream. */
+ * restores the handle's own stream, which is ordered with no other. (The default
+ * stream, number 0 to other libraries, is therefore given as cudaStreamLegacy.) */
 wg_status wg_device_set_stream(wg_device *dev, void *stream);
 /* Waits until the handle's stream is idle. */
 wg_status wg_device_sync(wg_device *dev);
@@ -399,7 +400,9 @@ wg_status wg_dgemv_dev(wg_device *dev, int trans, int64_t m, int64_t n, double a
  * 16-byte aligned and whose rows (and strideB) are whole 16-byte units are read
  * in place; others are first copied (of B, the matrices of groups with rows) to
  * memory of their size from the handle's stream-ordered pool (a call captured
- * into a graph has its own). Queued on the device stream. gpu_ms as for wg_sgemm. */
+ * into a graph has its own). Queued on the handle's stream (wg_device_set_stream):
+ * memory that other streams write or read is ordered with it by the caller. gpu_ms as
+ * for wg_sgemm. */
 #define WG_TYPE_F32 0
 #define WG_TYPE_BF16 1
 #define WG_TYPE_F16 2
@@ -434,7 +437,7 @@ wg_status wg_gemm_grouped_inner_dev(wg_device *dev, int type, int ctype, int64_t
  * A batch of matrices is stored one after the other in both. A matrix whose rows
  * are grouped (offsets as above) begins each group's scales at a new tile row,
  * so its scales have up to ceil(rows / 128) + groups tile rows; its codes are as
- * ever. All calls are queued on the device stream; gpu_ms as for wg_sgemm.
+ * ever. All calls are queued on the handle's stream; gpu_ms as for wg_sgemm.
  *
  * Quantises op(X), rows x cols (X stored rows x cols, or cols x rows when trans;
  * type WG_TYPE_F32, _BF16 or _F16; batch matrices strideX apart): for each block

@@ -84,8 +84,12 @@ class Device:
         return s.value or 0
 
     def set_stream(self, stream: int | None) -> None:
-        """Orders this device's work on a caller-owned stream (None: its own)."""
-        nat.check(nat.lib.wg_device_set_stream(self.handle, ct.c_void_p(stream or None)))
+        """Orders this device's work on a caller's stream, given as its cudaStream_t number, the
+        way other libraries name it (``torch.cuda.current_stream().cuda_stream``). 0 and 1 are
+        the legacy default stream, on which torch works unless told otherwise; None goes back to
+        the device's own stream, which is ordered with no other."""
+        # (to the C ABI NULL is the handle's own stream)
+        nat.check(nat.lib.wg_device_set_stream(self.handle, None if stream is None else ct.c_void_p(int(stream) or 1)))
 
     def synchronize(self) -> None:
         nat.check(nat.lib.wg_device_sync(self.handle))

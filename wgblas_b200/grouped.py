@@ -22,6 +22,10 @@ stream (``GpuArray.read`` or ``device.synchronize()`` waits for it), except on
 a benchmark device, which waits and returns ``gpuTimeMs``; and errors that only
 the device can see (offsets that decrease or leave the rows: they are clamped) are
 raised by ``device.check()``.
+
+CUDA tensors must be ordered on the device's stream: call
+``device.set_stream(torch.cuda.current_stream().cuda_stream)`` first. A device's own stream
+waits for no work of another library, nor that work for it.
 """
 from __future__ import annotations
 
@@ -91,6 +95,7 @@ def gemmGrouped(device, transB, groups, m, n, k, alpha, A, lda, B, ldb, strideB,
 
     A is m x k, C m x n, B_g (``strideB`` elements apart; 0 shares one matrix) k x n for
     "no-transpose" or n x k for "transpose". Rows that no group holds keep their C.
+    Queued on the device's stream, on which CUDA tensors must be ordered (``set_stream``).
     """
     st = nat._fast.gemm_grouped(device, transB, groups, m, n, k, alpha, A, lda, B, ldb, strideB, offsets, beta, C, ldc)
     if st is not None:  # the ordinary call, checked and made
@@ -140,6 +145,7 @@ def gemmGroupedInner(device, groups, m, n, k, alpha, A, lda, B, ldb, offsets, be
 
     A is k x m, B k x n, C_g (``strideC`` elements apart) m x n; ``offsets`` groups the k rows.
     A group without rows gives beta * C_g.
+    Queued on the device's stream, on which CUDA tensors must be ordered (``set_stream``).
     """
     st = nat._fast.gemm_grouped_inner(device, groups, m, n, k, alpha, A, lda, B, ldb, offsets, beta, C, ldc, strideC)
     if st is not None:

@@ -18,8 +18,9 @@ the groups' ``offsets`` and ``mxGemmGrouped`` multiplies by a batch of matrices;
 gradient of grouped weights, whose contraction is ragged, is ``gemmGroupedInner``'s.
 
 Like ``gemmGrouped``, the calls take flat resident arrays read as row-major
-matrices, are queued on the device's stream, and report what only the device can
-see (bad offsets) at ``device.check()``. The reference has no counterpart.
+matrices, are queued on the device's stream, on which CUDA tensors must be ordered
+(``device.set_stream``), and report what only the device can see (bad offsets) at
+``device.check()``. The reference has no counterpart.
 """
 from __future__ import annotations
 
@@ -149,6 +150,7 @@ def mxQuantize(device, trans, rows, cols, X, ldx, out, offsets=None, strideX=0):
     after the other). For each block the scale is 2^(floor(log2 max|x|) - 2), at least
     2^-127; elements are rounded to nearest, ties to even, beyond 6 scales to 6. A block
     with a NaN or an infinity becomes NaN.
+    Queued on the device's stream, on which CUDA tensors must be ordered (``set_stream``).
     """
     st = nat._fast.mx_quantize(device, trans, rows, cols, X, ldx, out, offsets, strideX)
     if st is not None:  # the ordinary call, checked and made
@@ -190,6 +192,7 @@ def mxDequantize(device, x, out, ldo, offsets=None, strideO=0):
 
     The matrices of a batch go ``strideO`` elements apart (by default one after the
     other). Rows that no group holds are not written.
+    Queued on the device's stream, on which CUDA tensors must be ordered (``set_stream``).
     """
     st = nat._fast.mx_dequantize(device, x, out, ldo, offsets, strideO)
     if st is not None:
@@ -254,6 +257,7 @@ def mxGemm(device, m, n, k, alpha, A, B, beta, C, ldc):
     """C := alpha * A B^T + beta * C with A (m x k) and B (n x k) in MXFP4.
 
     C is float32, bfloat16 or float16; sums are held in 32 bits.
+    Queued on the device's stream, on which CUDA tensors must be ordered (``set_stream``).
     """
     st = nat._fast.mx_gemm(device, 0, m, n, k, alpha, A, B, None, beta, C, ldc)
     if st is not None:
@@ -270,6 +274,7 @@ def mxGemmGrouped(device, groups, m, n, k, alpha, A, B, offsets, beta, C, ldc):
 
     A is m x k with rows grouped by ``offsets`` (quantised with the same ones), B a batch
     of ``groups`` n x k matrices. Rows that no group holds keep their C.
+    Queued on the device's stream, on which CUDA tensors must be ordered (``set_stream``).
     """
     if groups:
         st = nat._fast.mx_gemm(device, groups, m, n, k, alpha, A, B, offsets, beta, C, ldc)
