@@ -30,12 +30,18 @@ using wgg::WAIT_BUDGET;
 
 constexpr int BK = 64;          // k-block: 64 16-bit elements, one 128-byte swizzle span
 constexpr int EPI_WARPS = wgg::EPI_WARPS;
-// fp32 results: the tensor core truncates when it adds to the accumulator, about
-// 1e-9 of the result a contraction row (measured on normal data: 1.0e-6 at 1024
-// rows, 9.1e-6 at 8192). So accumulators are drained every SEG k-blocks and the
-// drained sums added in registers, rounded to nearest. 16-bit results round at
-// 2^-9 or 2^-11 and need no more than one accumulator.
-constexpr int SEG = 8;
+// The tensor core truncates when it adds to the accumulator: on data of one sign up to
+// 5.9e-9 of the sum a contraction row (measured, fp16 and bf16 values spread over
+// [0.5, 1.5]; normal data 1.2e-9). So accumulators are drained every so many k-blocks and
+// the drained sums added in registers, rounded to nearest:
+//   SEG   fp32 results (at most 2.4e-6 of a sum is lost to truncation), split contractions;
+//   LONG  16-bit results: 8192 rows, 4.8e-5, a tenth of fp16's half step (2^-11). bf16's
+//         (2^-8) is eight times that, so its sums are drained beyond 65536 rows only.
+// (An fp16 weight gradient of 2048 x 4096 over 16384 rows in 8 groups takes 169 us so, 165
+// from one accumulator.)
+constexpr int SEG = 8, LONG = 128;
+// Rows of a 16-bit result's contraction that one accumulator takes whole.
+constexpr int whole_rows(int type) { return type == WG_TYPE_BF16 ? 8 * LONG * BK : LONG * BK; }
 constexpr int CHUNK = 8192;     // bytes of 64 lines of one k-block
 constexpr size_t SMEM_LIMIT = 227 * 1024;
 
@@ -193,7 +199,7 @@ __device__ __forceinline__ void zero_end(uint8_t *st, int left, int chunks, int 
   __syncwarp();
 }
 
-// SUMS: accumulators are drained every SEG k-blocks (fp32 results).
+// DRAIN: k-blocks after which an accumulator is drained (SEG, LONG; 0: at the tile's end).
 // Warps: 0 and 10 load (the L and the N side), 1 issues the MMAs, 2-9 store, 11
 // (inner form) zeroes what is past a group's last row. That a group ends inside
 // the 16 lines of an MMA is known when its tile begins: those lines go to a place
@@ -201,7 +207,7 @@ __device__ __forceinline__ void zero_end(uint8_t *st, int left, int chunks, int 
 // that landing, zeroing and (in a pair) telling the other CTA are out of the way.
 // (With the last block zeroed in the ring they cost 27 us of 145 at 8192 rows in
 // 8 groups, 2048 x 4096 results.)
-template <int MODE, class S, bool SUMS>
+template <int MODE, class S, int DRAIN>
 __global__ void __launch_bounds__(MODE == INNER ? 384 : 352, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n,
                const __grid_constant__ CUtensorMap map_el, const __grid_constant__ CUtensorMap map_en, const Args a) {
@@ -366,7 +372,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       wgg::Ring<STAGES> ring;
       wgg::Ring<ENDS> ends;
       int used = 0;
-      constexpr int segment = SUMS ? SEG : 1 << 30;
+      constexpr int segment = DRAIN ? DRAIN : 1 << 30;
       constexpr uint64_t step_l = (L_MN ? 2048 : 32) >> 4, step_n = (N_MN ? 2048 : 32) >> 4;
       const uint32_t smem0 = wgtc::smem_addr(smem);
       const uint64_t desc_l0 = L_MN ? smem_desc_mn(smem0) : wgtc::smem_desc_kmajor(smem0, 128);
@@ -449,11 +455,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       const int64_t row = (MODE == INNER ? x.n0 : x.r0) + h * S::CPT;
       const int64_t at = (MODE == INNER ? (int64_t)x.g * a.strideC : 0) + row * a.out.ldc + l;
       const uint32_t col = tmem + (uint32_t)(h * S::CPT) + ((uint32_t)(q * 32) << 16);
-      if constexpr (SUMS || S::P > 1) {
+      if constexpr (DRAIN) {
         float sum[S::CPT];
 #pragma unroll
         for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
-        for (int kb0 = x.k_lo; kb0 < x.k_hi || (kb0 == x.k_lo && x.end); kb0 += SUMS ? SEG : 1 << 30) {
+        for (int kb0 = x.k_lo; kb0 < x.k_hi || (kb0 == x.k_lo && x.end); kb0 += DRAIN) {
           const int b = used & 1;
           if (!(ok = wait_acc(b))) break;
           wgg::drain<S::CPT>(col + (uint32_t)(b * S::BN), valid, kb0 == x.k_lo, sum);
@@ -470,7 +476,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
             break;
           }
         }
-        if (mine) wgg::store_sums<S::CPT, SUMS && S::P == 1>(a.out, at, l < a.nl, valid, sum);
+        if (mine) wgg::store_sums<S::CPT, DRAIN == SEG && S::P == 1>(a.out, at, l < a.nl, valid, sum);
       } else {
         const int b = used & 1;
         if (x.any && !(ok = wait_acc(b))) break;
@@ -604,7 +610,7 @@ bool make_maps(const Args &a, int type, CUtensorMap *ml, CUtensorMap *mn, CUtens
   return encode(ml, type, a.L, 3, dl, sl, bl) && encode(mn, type, a.N, 2, dn, &ldn, bn);
 }
 
-template <int MODE, class S, bool SUMS>
+template <int MODE, class S, int DRAIN>
 wg_status launch_as(wg_device *d, Args &a, const CUtensorMap (&m)[4]) {
   a.tiles_l = (a.nl + S::TL - 1) / S::TL;
   a.tiles_n = MODE == INNER ? (a.nn + S::BN - 1) / S::BN : 0;
@@ -612,8 +618,8 @@ wg_status launch_as(wg_device *d, Args &a, const CUtensorMap (&m)[4]) {
                                                            : (int64_t)a.rows / S::BN + a.groups);
   const unsigned grid = S::CLUSTER * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CLUSTER));
   wg_launch_scope scope(d, MODE == INNER ? "gemm_grouped_inner" : "gemm_grouped");
-  WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, SUMS>, SMEM_LIMIT));
-  WG_CUDA((wgg::launch<S::CLUSTER>(grouped_kernel<MODE, S, SUMS>, grid, MODE == INNER ? 384 : 352, S::smem(a.groups),
+  WG_CUDA(wg_kernel_smem(grouped_kernel<MODE, S, DRAIN>, SMEM_LIMIT));
+  WG_CUDA((wgg::launch<S::CLUSTER>(grouped_kernel<MODE, S, DRAIN>, grid, MODE == INNER ? 384 : 352, S::smem(a.groups),
                               d->stream, m[0], m[1], m[2], m[3], a)));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
@@ -626,11 +632,14 @@ wg_status launch(wg_device *d, Args &a, int type) {
   // (no product, no operands)
   if (a.out.alpha != 0.0f && !make_maps<MODE, S>(a, type, &m[0], &m[1], &m[2], &m[3]))
     return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
-  // One accumulator holds at most SEG k-blocks' sums of an fp32 result.
   // (a split contraction's sums are always drained, and few blocks long)
-  const bool sums = S::P > 1 || (a.out.type == WG_TYPE_F32 && (MODE == INNER ? a.rows : a.k) > SEG * BK);
-  if constexpr (S::P > 1) return launch_as<MODE, S, true>(d, a, m);
-  else return sums ? launch_as<MODE, S, true>(d, a, m) : launch_as<MODE, S, false>(d, a, m);
+  if constexpr (S::P > 1) {
+    return launch_as<MODE, S, SEG>(d, a, m);
+  } else {
+    const int rows = MODE == INNER ? a.rows : a.k;  // the longest contraction there can be
+    if (a.out.type == WG_TYPE_F32) return rows > SEG * BK ? launch_as<MODE, S, SEG>(d, a, m) : launch_as<MODE, S, 0>(d, a, m);
+    return rows > whole_rows(a.out.type) ? launch_as<MODE, S, LONG>(d, a, m) : launch_as<MODE, S, 0>(d, a, m);
+  }
 }
 
 // The form with the least modelled time. A form's tiles run in rounds over the

@@ -537,9 +537,15 @@ __global__ void __launch_bounds__(256) mx_dequantize_unaligned(const QuantArgs a
 constexpr int BKE = 256;           // elements of a k-block
 constexpr int EPI_WARPS = wgg::EPI_WARPS;
 constexpr size_t SMEM_LIMIT = 227 * 1024;
-// fp32 results: k-blocks between drains of the accumulator, whose additions
-// truncate (grouped.cu).
-constexpr int SEG = 16;
+// k-blocks between drains of the accumulator, whose additions truncate (grouped.cu): up
+// to 3e-10 of the sum a contraction row here (measured at 2^19 rows, positive values over
+// many powers of two; sums of values alike are exact for longer). SEG: fp32 results and
+// split contractions. LONG: 16-bit results, 65536 rows, 1024 MMAs that lose at most 2^-23 of a
+// partial sum each, 6.1e-5 of the whole: an eighth of fp16's half step (2^-11). bf16's
+// (2^-8) is eight times that, so its sums are drained beyond 524288 rows only.
+constexpr int SEG = 16, LONG = 256;
+// Rows of a 16-bit result's contraction that one accumulator takes whole.
+constexpr int whole_rows(int type) { return type == WG_TYPE_BF16 ? 8 * LONG * BKE : LONG * BKE; }
 
 // CG CTAs (a pair or one) share a tile's lanes, P CTAs its contraction.
 template <int CG_, int BN_, int P_ = 1>
@@ -643,8 +649,9 @@ __device__ __forceinline__ Tile tile_at(const Args &a, int64_t t, const int *sta
 }
 
 // Warps: 0 and 10 load (the L and the N side, codes and scales), 1 issues the
-// MMAs, 2-9 store. SUMS: the accumulator is drained every SEG k-blocks.
-template <class S, bool SUMS>
+// MMAs, 2-9 store. DRAIN: k-blocks after which the accumulator is drained (SEG, LONG; 0:
+// at the tile's end).
+template <class S, int DRAIN>
 __global__ void __launch_bounds__(352, 1)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant__ CUtensorMap map_n,
                const __grid_constant__ CUtensorMap map_sl, const __grid_constant__ CUtensorMap map_sn, const Args a) {
@@ -747,7 +754,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       wgg::Ring<STAGES> ring;
       int used = 0;
       uint32_t set = 0;  // which set of scale columns
-      constexpr int segment = SUMS ? SEG : 1 << 30;
+      constexpr int segment = DRAIN ? DRAIN : 1 << 30;
       const uint32_t smem0 = wgtc::smem_addr(smem);
       const uint64_t desc_l0 = wgtc::smem_desc_kmajor(smem0, 128);
       const uint64_t desc_n0 = wgtc::smem_desc_kmajor(smem0 + S::L_BYTES, 128);
@@ -811,7 +818,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       float sum[S::CPT];
 #pragma unroll
       for (int j = 0; j < S::CPT; j++) sum[j] = 0.0f;
-      for (int kb0 = x.k_lo; kb0 < x.k_hi; kb0 += SUMS ? SEG : 1 << 30, used++) {
+      for (int kb0 = x.k_lo; kb0 < x.k_hi; kb0 += DRAIN ? DRAIN : 1 << 30, used++) {
         const int b = used % S::ACCS;
         ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_full[b], (uint32_t)(used / S::ACCS) & 1u, WAIT_BUDGET) &&
                                          *abort_flag == 0);
@@ -836,7 +843,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
           break;
         }
       }
-      if (mine) wgg::store_sums<S::CPT, SUMS && S::P == 1>(a.out, at, l < a.n, valid, sum);
+      if (mine) wgg::store_sums<S::CPT, DRAIN == SEG && S::P == 1>(a.out, at, l < a.n, valid, sum);
     }
   }
 
@@ -924,13 +931,13 @@ struct Operands {
   const uint8_t *A, *As, *B, *Bs;
 };
 
-template <class S, bool SUMS>
+template <class S, int DRAIN>
 wg_status launch_as(wg_device *d, const char *family, Args &a, const CUtensorMap (&m)[4]) {
   const int64_t most = ((int64_t)a.rows / S::BN + a.groups) * a.tiles_l;
   const unsigned grid = S::CLUSTER * (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, d->sm_count / S::CLUSTER));
   wg_launch_scope scope(d, family);
-  WG_CUDA(wg_kernel_smem(mx_gemm_kernel<S, SUMS>, SMEM_LIMIT));
-  WG_CUDA((wgg::launch<S::CLUSTER>(mx_gemm_kernel<S, SUMS>, grid, 352, S::smem(a.groups), d->stream, m[0], m[1], m[2], m[3], a)));
+  WG_CUDA(wg_kernel_smem(mx_gemm_kernel<S, DRAIN>, SMEM_LIMIT));
+  WG_CUDA((wgg::launch<S::CLUSTER>(mx_gemm_kernel<S, DRAIN>, grid, 352, S::smem(a.groups), d->stream, m[0], m[1], m[2], m[3], a)));
   WG_CUDA(cudaGetLastError());
   return WG_OK;
 }
@@ -957,9 +964,12 @@ wg_status launch_gemm(wg_device *d, const char *family, Args &a, const Operands 
         !encode(&m[2], u32, o.Bs, 2, dsl, &ss, bsl, no) || !encode(&m[3], u32, o.As, 2, dsn, &ss, bsn, no))
       return wg_fail(WG_ERR_INVALID_ARGUMENT, "the operands' sizes exceed what a tensor map describes");
   }
-  if constexpr (S::P > 1) return launch_as<S, true>(d, family, a, m);
-  else return a.out.type == WG_TYPE_F32 && a.k > SEG * BKE ? launch_as<S, true>(d, family, a, m)
-                                                          : launch_as<S, false>(d, family, a, m);
+  if constexpr (S::P > 1) {
+    return launch_as<S, SEG>(d, family, a, m);
+  } else {
+    if (a.out.type == WG_TYPE_F32) return a.k > SEG * BKE ? launch_as<S, SEG>(d, family, a, m) : launch_as<S, 0>(d, family, a, m);
+    return a.k > whole_rows(a.out.type) ? launch_as<S, LONG>(d, family, a, m) : launch_as<S, 0>(d, family, a, m);
+  }
 }
 
 // The form with the least modelled time, as for the 16-bit products (grouped.cu);
