@@ -242,7 +242,11 @@ __device__ __forceinline__ void store_acc(uint32_t taddr, bool from, const Out &
 // Their epilogue warps write them into its shared memory, [part][column][lane],
 // when its warps have read the last tile's. The writes are asynchronous and count
 // themselves on CTA 0's barrier as they land, so nobody has to make them visible
-// (a release at cluster scope took about a thousand clocks).
+// (a release at cluster scope behind a warp's own stores took about a thousand clocks);
+// CTA 0 acquires them by waiting at cluster scope. Its arrivals that give the place back
+// release its warps' reads at cluster scope, the others' waits acquire them; that release
+// is not free either (0.2 us of 8 for 4 x 512 x 4096 in 8 groups) and left out where no
+// further tile can ask for the place.
 
 struct Parts {
   float *buf;        // CTA 0: (P - 1) x BN x 128 sums
@@ -253,15 +257,15 @@ struct Parts {
 
 // Joins sum[] over the cluster; true on CTA 0, which then holds the total. A warp
 // of CTA `rank` calls it with its columns' place (`col` of the tile, lane `row`)
-// and the tile's number of columns; `first`: the one warp that announces the bytes.
-// False with *ok = false when a wait gave up.
+// and the tile's number of columns; `first`: the one warp that announces the bytes;
+// `more`: the cluster has tiles after this one. False with *ok = false when a wait gave up.
 template <int P, int BN, int CPT>
 __device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int row, int valid, int columns, bool first,
-                                           float (&sum)[CPT], bool *ok) {
+                                           bool more, float (&sum)[CPT], bool *ok) {
   const uint32_t turn = x.turn++;
   const int lane = threadIdx.x & 31;
   if (rank) {
-    if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded(x.empty, (turn & 1u) ^ 1u, WAIT_BUDGET))) {
+    if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(x.empty, (turn & 1u) ^ 1u, WAIT_BUDGET))) {
       *ok = false;
       return false;
     }
@@ -276,7 +280,7 @@ __device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int
     return false;
   }
   if (first && lane == 0) wgtc::mbar_arrive_expect_tx(x.full, (uint32_t)((P - 1) * columns * BL * 4));
-  if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded(x.full, turn & 1u, WAIT_BUDGET))) {
+  if (!__all_sync(0xffffffffu, wgtc::mbar_wait_bounded_cluster(x.full, turn & 1u, WAIT_BUDGET))) {
     *ok = false;
     return false;
   }
@@ -288,11 +292,8 @@ __device__ __forceinline__ bool join_parts(Parts &x, uint32_t rank, int col, int
       if (j < valid) sum[j] += from[128 * j];
   }
   __syncwarp();
-  // (the sums are in registers: the arrival orders nothing else)
-  if (lane > 0 && lane < P)
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
-                     wgtc::mapa_shared(wgtc::smem_addr(x.empty), (uint32_t)lane))
-                 : "memory");
+  if (more && lane > 0 && lane < P)
+    wgtc::mbar_arrive_cluster(wgtc::mapa_shared(wgtc::smem_addr(x.empty), (uint32_t)lane));
   return true;
 }
 

@@ -836,7 +836,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       bool mine = true;
       if constexpr (S::P > 1) {
         if (kt) mine = wgg::join_parts<S::P, S::BN, S::CPT>(parts, rank, h * S::CPT, q * 32 + lane, valid, x.nv,
-                                                              warp == 2, sum, &ok);
+                                                              warp == 2, t + t_step < tiles, sum, &ok);
         else mine = rank == 0;
         if (!ok) {
           if (lane == 0) gave_up(WG_DERR_MMA_WAIT);
