@@ -50,7 +50,7 @@ class GpuMxMatrix:
     include/wgblas.h: rows of two elements a byte, and tiles of 128 rows x 4 scale bytes.
     """
 
-    __slots__ = ("device", "rows", "cols", "batch", "groups", "codes", "scales", "_codes", "_scales")
+    __slots__ = ("device", "rows", "cols", "batch", "groups", "codes", "scales", "_codes", "_scales", "_owned")
 
     def __init__(self, device, codes, scales, rows, cols, batch, groups):
         self.device = device
@@ -88,7 +88,9 @@ class GpuMxMatrix:
         except Exception:
             codes.destroy()
             raise
-        return GpuMxMatrix(device, codes, scales, rows, cols, batch, groups)
+        x = GpuMxMatrix(device, codes, scales, rows, cols, batch, groups)
+        x._owned = True
+        return x
 
     @staticmethod
     def wrap(device, codes, scales, rows, cols, batch=1, groups=0) -> "GpuMxMatrix":
@@ -100,9 +102,9 @@ class GpuMxMatrix:
 
     def destroy(self) -> None:
         """Frees arrays made by ``empty`` (wrapped memory is the caller's)."""
-        for x in (self.codes, self.scales):
-            if isinstance(x, GpuArray):
-                x.destroy()
+        if getattr(self, "_owned", False):  # (only ``empty`` sets it)
+            self.codes.destroy()
+            self.scales.destroy()
         self._codes = self._scales = 0
         self.rows = self.cols = 0
 
