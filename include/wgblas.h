@@ -395,7 +395,7 @@ wg_status wg_dgemv_dev(wg_device *dev, int trans, int64_t m, int64_t n, double a
  * to the range and to the largest before it) and reported by wg_device_check.
  *
  * alpha, beta as for wg_sgemm: alpha == 0 reads neither A nor B, beta == 0 does
- * not read C. C must not overlap A or B. Pointers, leading dimensions and
+ * not read C. C must not overlap A, B or the offsets. Pointers, leading dimensions and
  * strides need only the alignment of their elements: operands whose bases are
  * 16-byte aligned and whose rows (and strideB) are whole 16-byte units are read
  * in place; others are first copied (of B, the matrices of groups with rows) to
@@ -437,7 +437,8 @@ wg_status wg_gemm_grouped_inner_dev(wg_device *dev, int type, int ctype, int64_t
  * A batch of matrices is stored one after the other in both. A matrix whose rows
  * are grouped (offsets as above) begins each group's scales at a new tile row,
  * so its scales have up to ceil(rows / 128) + groups tile rows; its codes are as
- * ever. All calls are queued on the handle's stream; gpu_ms as for wg_sgemm.
+ * ever. No result may overlap an operand or the offsets. All calls are queued on the
+ * handle's stream; gpu_ms as for wg_sgemm.
  *
  * Quantises op(X), rows x cols (X stored rows x cols, or cols x rows when trans;
  * type WG_TYPE_F32, _BF16 or _F16; batch matrices strideX apart): for each block

@@ -196,6 +196,10 @@ static int64_t plus(int64_t a, int64_t count, int64_t stride) {
 static int apart(uintptr_t p, int64_t bytes, uintptr_t q, int64_t qbytes) {
   return !(p < q + (uintptr_t)qbytes && q < p + (uintptr_t)bytes);
 }
+/* No offsets, or none of them in the range: CTAs read them at different times. */
+static int apart_offsets(uintptr_t p, int64_t bytes, const int *offsets, int64_t groups) {
+  return !offsets || apart(p, bytes, (uintptr_t)offsets, (groups + 1) * 4);
+}
 static int64_t codes_size(int64_t rows, int64_t cols, int64_t batch) {
   const __int128 v = (__int128)batch * rows * ((cols + 31) / 32 * 16);
   return v < ((__int128)1 << 61) ? (int64_t)v : -1;
@@ -235,7 +239,8 @@ static PyObject *gemm_grouped(PyObject *self, PyObject *const *v, Py_ssize_t nv)
       A.n < ua || B.n < ub || C.n < uc || O.n < groups + 1)
     Py_RETURN_NONE;
   const int64_t cb = uc * item_bytes[C.type];
-  if (!apart(C.p, cb, A.p, ua * 2) || !apart(C.p, cb, B.p, ub * 2)) Py_RETURN_NONE;
+  if (!apart(C.p, cb, A.p, ua * 2) || !apart(C.p, cb, B.p, ub * 2) || !apart_offsets(C.p, cb, (const int *)O.p, groups))
+    Py_RETURN_NONE;
   wg_status st;
   Py_BEGIN_ALLOW_THREADS
   st = wg_gemm_grouped_dev(d.handle, A.type, C.type, trans, groups, m, n, k, alpha, (const void *)A.p, lda,
@@ -267,7 +272,8 @@ static PyObject *gemm_grouped_inner(PyObject *self, PyObject *const *v, Py_ssize
       (groups > 1 && strideC < one) || A.n < ua || B.n < ub || C.n < uc || O.n < groups + 1)
     Py_RETURN_NONE;
   const int64_t cb = uc * item_bytes[C.type];
-  if (!apart(C.p, cb, A.p, ua * 2) || !apart(C.p, cb, B.p, ub * 2)) Py_RETURN_NONE;
+  if (!apart(C.p, cb, A.p, ua * 2) || !apart(C.p, cb, B.p, ub * 2) || !apart_offsets(C.p, cb, (const int *)O.p, groups))
+    Py_RETURN_NONE;
   wg_status st;
   Py_BEGIN_ALLOW_THREADS
   st = wg_gemm_grouped_inner_dev(d.handle, A.type, C.type, groups, m, n, k, alpha, (const void *)A.p, lda,
@@ -310,7 +316,8 @@ static PyObject *mx_quantize(PyObject *self, PyObject *const *v, Py_ssize_t nv) 
   const int64_t used = plus(span(srows, scols, ldx), out.batch - 1, strideX);
   const int64_t nc = codes_size(rows, cols, out.batch), ns = scales_size(rows, cols, out.batch, out.groups);
   if (ldx < scols || used < 0 || X.n < used || nc < 0 || ns < 0) Py_RETURN_NONE;
-  if (!apart(out.codes, nc, X.p, used * item_bytes[X.type]) || !apart(out.scales, ns, X.p, used * item_bytes[X.type]))
+  if (!apart(out.codes, nc, X.p, used * item_bytes[X.type]) || !apart(out.scales, ns, X.p, used * item_bytes[X.type]) ||
+      !apart_offsets(out.codes, nc, off, out.groups) || !apart_offsets(out.scales, ns, off, out.groups))
     Py_RETURN_NONE;
   wg_status st;
   Py_BEGIN_ALLOW_THREADS
@@ -342,7 +349,8 @@ static PyObject *mx_dequantize(PyObject *self, PyObject *const *v, Py_ssize_t nv
   const int64_t nc = codes_size(x.rows, x.cols, x.batch), ns = scales_size(x.rows, x.cols, x.batch, x.groups);
   if (one < 0 || used < 0 || nc < 0 || ns < 0 || (x.batch > 1 && strideO < one) || O.n < used) Py_RETURN_NONE;
   const int64_t ob = used * item_bytes[O.type];
-  if (!apart(O.p, ob, x.codes, nc) || !apart(O.p, ob, x.scales, ns)) Py_RETURN_NONE;
+  if (!apart(O.p, ob, x.codes, nc) || !apart(O.p, ob, x.scales, ns) || !apart_offsets(O.p, ob, off, x.groups))
+    Py_RETURN_NONE;
   wg_status st;
   Py_BEGIN_ALLOW_THREADS
   st = wg_mx_dequantize_dev(d.handle, O.type, x.batch, x.rows, x.cols, (const void *)x.codes, (const void *)x.scales,
@@ -378,7 +386,7 @@ static PyObject *mx_gemm(PyObject *self, PyObject *const *v, Py_ssize_t nv) {
   if (used < 0 || C.n < used || ca < 0 || cb < 0 || sa < 0 || sb < 0) Py_RETURN_NONE;
   const int64_t bytes = used * item_bytes[C.type];
   if (!apart(C.p, bytes, A.codes, ca) || !apart(C.p, bytes, B.codes, cb) || !apart(C.p, bytes, A.scales, sa) ||
-      !apart(C.p, bytes, B.scales, sb))
+      !apart(C.p, bytes, B.scales, sb) || !apart_offsets(C.p, bytes, off, groups))
     Py_RETURN_NONE;
   wg_status st;
   Py_BEGIN_ALLOW_THREADS

@@ -135,7 +135,7 @@ def gemmGrouped(device, transB, groups, m, n, k, alpha, A, lda, B, ldb, strideB,
         need("A", na, use_a, "m, k, and lda")
         need("B", nb, use_b, "groups, n, k, ldb, and strideB")
     need("C", nc, use_c, "m, n, and ldc")
-    disjoint("C", (pc, use_c), tc, (("A", pa, use_a, ta), ("B", pb, use_b, tb)))
+    disjoint("C", (pc, use_c), tc, (("A", pa, use_a, ta), ("B", pb, use_b, tb), ("offsets", po, groups + 1, "int32")))
     return timed(device, nat.lib.wg_gemm_grouped_dev, device.handle, TYPE_CODES[ta], TYPE_CODES[tc], int(trans), groups,
                  m, n, k, alpha, pa, lda, pb, ldb, strideB, po, beta, pc, ldc)
 
@@ -180,7 +180,7 @@ def gemmGroupedInner(device, groups, m, n, k, alpha, A, lda, B, ldb, offsets, be
         need("A", na, use_a, "k, m, and lda")
         need("B", nb, use_b, "k, n, and ldb")
     need("C", nc, use_c, "groups, m, n, ldc, and strideC")
-    disjoint("C", (pc, use_c), tc, (("A", pa, use_a, ta), ("B", pb, use_b, tb)))
+    disjoint("C", (pc, use_c), tc, (("A", pa, use_a, ta), ("B", pb, use_b, tb), ("offsets", po, groups + 1, "int32")))
     return timed(device, nat.lib.wg_gemm_grouped_inner_dev, device.handle, TYPE_CODES[ta], TYPE_CODES[tc], groups, m, n,
                  k, alpha, pa, lda, pb, ldb, po, beta, pc, ldc, strideC)
 

@@ -144,6 +144,10 @@ def _mx_ranges(x):
             ("scales", x._scales, mxScalesSize(x.rows, x.cols, x.batch, x.groups), "uint8"))
 
 
+def _offsets_range(x, ptr):
+    return (("offsets", ptr, x.groups + 1, "int32"),) if x.groups else ()
+
+
 def mxQuantize(device, trans, rows, cols, X, ldx, out, offsets=None, strideX=0):
     """out := op(X) in MXFP4; out is rows x cols, its blocks of 32 run along its rows.
 
@@ -184,7 +188,7 @@ def mxQuantize(device, trans, rows, cols, X, ldx, out, offsets=None, strideX=0):
     used += (out.batch - 1) * strideX
     need("X", nx, used, "rows, cols, ldx, and strideX")
     for name, p, n, kind in _mx_ranges(out):
-        disjoint("out", (p, n), kind, (("X", px, used, tx),))
+        disjoint("out", (p, n), kind, (("X", px, used, tx), *_offsets_range(out, po)))
     return timed(device, nat.lib.wg_mx_quantize_dev, device.handle, TYPE_CODES[tx], int(t), out.batch, rows, cols, px, ldx,
                  strideX, out.groups, po, out._codes, out._scales)
 
@@ -222,7 +226,7 @@ def mxDequantize(device, x, out, ldo, offsets=None, strideO=0):
         raise Error("strideO must be at least one matrix of out.")
     used += (x.batch - 1) * strideO
     need("out", no, used, "rows, cols, ldo, and strideO")
-    disjoint("out", (po, used), to, _mx_ranges(x))
+    disjoint("out", (po, used), to, (*_mx_ranges(x), *_offsets_range(x, off)))
     return timed(device, nat.lib.wg_mx_dequantize_dev, device.handle, TYPE_CODES[to], x.batch, rows, cols, x._codes,
                  x._scales, x.groups, off, po, ldo, strideO)
 
@@ -293,6 +297,7 @@ def mxGemmGrouped(device, groups, m, n, k, alpha, A, B, offsets, beta, C, ldc):
     po = check_offsets(device, "mxGemmGrouped", offsets, groups)
     if not used:
         return {}
+    disjoint("C", (pc, used), tc, _offsets_range(A, po))
     return timed(device, nat.lib.wg_mx_gemm_grouped_dev, device.handle, TYPE_CODES[tc], groups, m, n, k, alpha, A._codes,
                  A._scales, B._codes, B._scales, po, beta, pc, ldc)
 
