@@ -6,7 +6,9 @@ module without it raises ImportError — there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as ct
+import importlib.util
 import os
+import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libwgblas_b200.so")
@@ -17,7 +19,29 @@ if not os.path.exists(LIB_PATH):
         "(wgblas_b200 has no CPU fallback)")
 
 lib = ct.CDLL(LIB_PATH)
-from . import _fast  # noqa: E402  (csrc/fastcall.c, built with the library; it calls the library loaded above)
+
+
+class _NoFast:
+    """In place of the fast path: handles no call, so that every one takes the Python checks."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _load_fast():
+    """csrc/fastcall.c as built for this very interpreter (build.py names the file by its ABI tag; it
+    calls the library loaded above), or a stand-in that leaves every call to the Python checks."""
+    path = os.path.join(_HERE, "_fast" + sysconfig.get_config_var("EXT_SUFFIX"))
+    if not os.path.exists(path):
+        return _NoFast()
+    spec = importlib.util.spec_from_file_location(__package__ + "._fast", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+_fast = _load_fast()
+has_fast = not isinstance(_fast, _NoFast)
 
 # status codes (wg_status)
 WG_OK = 0

@@ -5,6 +5,7 @@ Usage: python wgblas_b200/build.py [--force] [-v]   (runs without importing the 
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -57,16 +58,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 FAST_SRC = os.path.join(CSRC, "fastcall.c")
-FAST = os.path.join(HERE, "_fast.so")
+# (object slots are read by offset: the file is this interpreter's and no other's)
+FAST = os.path.join(HERE, "_fast" + sysconfig.get_config_var("EXT_SUFFIX"))
+PYTHON_INCLUDE = sysconfig.get_paths()["include"]
 
 
-def build_fast(force: bool = False) -> str:
-    """Builds the CPython extension _fast (csrc/fastcall.c) next to the library it calls."""
-    if force or _stale(FAST, [FAST_SRC, LIB, os.path.join(ROOT, "include", "wgblas.h")]):
-        subprocess.run(["gcc", "-std=c11", "-O2", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
-                        "-fvisibility=hidden", "-I" + os.path.join(ROOT, "include"),
-                        "-I" + sysconfig.get_paths()["include"], FAST_SRC, "-L" + HERE, "-lwgblas_b200",
-                        "-Wl,-rpath,$ORIGIN", "-o", FAST], check=True)
+def build_fast(force: bool = False) -> str | None:
+    """Builds the CPython extension _fast (csrc/fastcall.c) next to the library it calls. Without a C
+    compiler or this interpreter's headers it is left out, and the package goes by its Python checks."""
+    if not force and not _stale(FAST, [FAST_SRC, LIB, os.path.join(ROOT, "include", "wgblas.h")]):
+        return FAST
+    cc, header = shutil.which("gcc"), os.path.join(PYTHON_INCLUDE, "Python.h")
+    if not cc or not os.path.exists(header) or sys.version_info < (3, 9):
+        print("_fast (csrc/fastcall.c) is not built: it needs gcc, Python >= 3.9 and " + header, file=sys.stderr)
+        return None
+    subprocess.run([cc, "-std=c11", "-O2", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
+                    "-fvisibility=hidden", "-I" + os.path.join(ROOT, "include"), "-I" + PYTHON_INCLUDE, FAST_SRC,
+                    "-L" + HERE, "-lwgblas_b200", "-Wl,-rpath,$ORIGIN", "-o", FAST], check=True)
     return FAST
 
 

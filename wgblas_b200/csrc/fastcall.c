@@ -8,10 +8,15 @@
  * pass every check. It returns the wg_status of the call then, and None for
  * anything else, without having called the library: the Python function of the
  * same name (grouped.py, mx.py) then goes through the same checks one by one and
- * raises or calls. Nothing is accepted here that is refused there.
+ * raises or calls. Nothing is accepted here that is refused there. The package does
+ * without this file where it was not built for the running interpreter.
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#if PY_VERSION_HEX < 0x030C0000
+#include <structmember.h>
+#define Py_T_OBJECT_EX T_OBJECT_EX
+#endif
 #include <stdint.h>
 
 #include "wgblas.h"
