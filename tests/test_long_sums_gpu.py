@@ -180,3 +180,84 @@ def test_mx_in_32_bits(wg, dev, m):
     want = product64(x, x)
     assert (c.double() - want).norm() <= 1.6e-5 * want.norm()
     q.destroy()
+
+
+# ---- the longest contractions a call takes ---------------------------------------------------
+# (a wait for one accumulator's whole contraction would pass the kernels' time limit of 4e9 clocks
+# here: 2^25 k-blocks take 230 clocks each)
+
+
+def needs(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of free device memory")
+
+
+@pytest.mark.parametrize("groups", [1, 200], ids=["split", "whole"])
+def test_as_many_contraction_rows_as_a_call_takes(wg, dev, groups):
+    """One group has them all, in a call that splits its contraction and in one that does not."""
+    needs(72)
+    k, m, n = (1 << 31) - 1025, 8, 8
+    a, b = (torch.zeros((k, s), dtype=torch.bfloat16, device="cuda") for s in (m, n))
+    want = torch.zeros((m, n), dtype=torch.float64, device="cuda")
+    for i, r in enumerate((slice(0, 300), slice(1 << 30, (1 << 30) + 500), slice(k - 77, k))):
+        for x in (a, b):
+            x[r] = positive((r.stop - r.start, m), torch.bfloat16, 10 + i)
+        want += a[r].double().t() @ b[r].double()
+    off = torch.full((groups + 1,), k, dtype=torch.int32, device="cuda")
+    off[: groups // 2 + 1] = 0
+    c = torch.full((groups, m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    wg.gemmGroupedInner(dev, groups, m, n, k, 2.0 ** -4, a, m, b, n, off, 0.0, c, n, m * n)
+    dev.check()
+    check(c[groups // 2], want / 16, "bfloat16")
+    c[groups // 2] = 0
+    assert (c == 0).all()
+    del a, b
+    torch.cuda.empty_cache()
+
+
+def test_a_ragged_group_behind_a_very_long_one(wg, dev):
+    """Two tiles of one CTA, both with rows past the last whole 16: the second's wait for its last rows
+    takes as long as the first's contraction."""
+    needs(72)
+    first, second, m, n = (3 << 29) + 5, (1 << 26) + 7, 8, 8
+    groups, other = 200, torch.cuda.get_device_properties(0).multi_processor_count
+    k = first + second
+    a, b = (torch.zeros((k, s), dtype=torch.bfloat16, device="cuda") for s in (m, n))
+    wants = []
+    for i, ends in enumerate(((0, first), (first, k))):
+        spots = slice(ends[0], ends[0] + 300), slice(ends[1] - 77, ends[1])
+        for x in (a, b):
+            for r in spots:
+                x[r] = positive((r.stop - r.start, m), torch.bfloat16, 30 + i)
+        wants.append(sum(a[r].double().t() @ b[r].double() for r in spots))
+    off = torch.full((groups + 1,), first, dtype=torch.int32, device="cuda")
+    off[0], off[other + 1:] = 0, k
+    c = torch.full((groups, m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    wg.gemmGroupedInner(dev, groups, m, n, k, 2.0 ** -4, a, m, b, n, off, 0.0, c, n, m * n)
+    dev.check()
+    for g, want in zip((0, other), wants):
+        check(c[g], want / 16, "bfloat16")
+        c[g] = 0
+    assert (c == 0).all()
+    del a, b
+    torch.cuda.empty_cache()
+
+
+def test_as_many_columns_as_an_mx_call_takes(wg, dev):
+    needs(72)
+    k, m = (1 << 31) - 1025, 8
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    spots = (slice(0, 300), slice(1 << 30, (1 << 30) + 512), slice(k - 77, k))
+    for i, r in enumerate(spots):
+        x[:, r] = positive((m, r.stop - r.start), torch.bfloat16, 20 + i)
+    q = wg.GpuMxMatrix.empty(dev, m, k)
+    wg.mxQuantize(dev, N, m, k, x, k, q)
+    wg.mxDequantize(dev, q, x, k)
+    c = torch.zeros((m, m), dtype=torch.bfloat16, device="cuda")
+    wg.mxGemm(dev, m, m, k, 2.0 ** -4, q, q, 0.0, c, m)
+    dev.check()
+    want = sum(x[:, r].double() @ x[:, r].double().t() for r in spots)
+    check(c, want / 16, "bfloat16")
+    q.destroy()
+    del x
+    torch.cuda.empty_cache()

@@ -42,6 +42,7 @@ constexpr int EPI_WARPS = wgg::EPI_WARPS;
 constexpr int SEG = 8, LONG = 128;
 // Rows of a 16-bit result's contraction that one accumulator takes whole.
 constexpr int whole_rows(int type) { return type == WG_TYPE_BF16 ? 8 * LONG * BK : LONG * BK; }
+constexpr long long BLOCK_BUDGET = 5000;  // clocks a k-block may take (230 to 512 where nothing delays it)
 constexpr int CHUNK = 8192;     // bytes of 64 lines of one k-block
 constexpr size_t SMEM_LIMIT = 227 * 1024;
 
@@ -343,13 +344,22 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
       if (!wgtc::mbar_wait_bounded(&end_empty[ends.s], ends.round ^ 1u, WAIT_BUDGET)) break;
   } else if (MODE == INNER && warp == 11) {
     // ---- ragged ends: zeroes the lines past a group's last row, then hands the place on ----
+    // Lines are loaded behind the k-blocks of the tiles before theirs, so a wait lasts as long
+    // as those take: 2^24 k-blocks pass the limit that the other waits have. This one's
+    // grows with them, by ten times what a k-block takes.
     wgg::Ring<ENDS> ends;
+    long long budget = WAIT_BUDGET;
     for (int64_t t = t_first; t < tiles; t += t_step) {
       const Tile x = tile_at<MODE, S>(a, t, start, tile0, rank);
-      if (!x.end) continue;
+      const long long blocks = x.k_hi - x.k_lo;
+      if (!x.end) {
+        budget += blocks * BLOCK_BUDGET;
+        continue;
+      }
       const int e = ends.s;
       const int nmma = (x.nv + S::NMMA_STEP - 1) & ~(S::NMMA_STEP - 1);
-      bool ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&end_here[e], ends.round, WAIT_BUDGET));
+      bool ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&end_here[e], ends.round, budget));
+      budget = WAIT_BUDGET + blocks * BLOCK_BUDGET;
       if (ok) {
         zero_end(smem + S::ends + (size_t)e * S::END, x.end, 2 + (nmma / CG + 63) / 64, lane);
         if (CG == 2 && half == 1) {
