@@ -80,3 +80,39 @@ def test_the_documented_step_is_ordered_with_torch(wg, side, n, k):
     one = np.ones((G, n, k))
     want, mag = gc.inner_form(ds, xs, ends, 1.0, 1.0, one)
     gc.assert_close(got[2].double().cpu().numpy(), want, mag, m, 1.0, one, "float32", "dW")
+
+
+@pytest.mark.gpu
+def test_the_other_routines_on_the_default_stream(wg):
+    """Host-array and resident calls give the same bits as on the handle's own stream."""
+    dev = wg.init()
+
+    def results():
+        out = []
+        for m, n, k in ((70, 50, 90), (640, 1100, 700), (2304, 2304, 2304)):
+            a, b = wg.randomNormalFloat32Array(m * k, 1), wg.randomNormalFloat32Array(k * n, 2)
+            c = np.zeros(m * n, np.float32)
+            out.append(wg.sgemm(dev, "no-transpose", "no-transpose", m, n, k, 1.5, a, k, b, n, 0.0, c, n)["C"])
+            ga, gb = (wg.GpuMatrix.from_(dev, v, r, s) for v, r, s in ((a, m, k), (b, k, n)))
+            gcm = wg.GpuMatrix.from_(dev, np.zeros(m * n, np.float32), m, n)
+            wg.sgemm(dev, "no-transpose", "no-transpose", m, n, k, 1.5, ga, k, gb, n, 0.0, gcm, n)
+            out.append(np.asarray(gcm.read()).copy())
+            for x in (ga, gb, gcm):
+                x.destroy()
+        n = 300
+        tri = np.tril(wg.randomNormalFloat32Array(n * n, 3).reshape(n, n)) + 20 * np.eye(n, dtype=np.float32)
+        tri = tri.astype(np.float32).reshape(-1)
+        rhs, x, y = wg.randomNormalFloat32Array(n * 40, 4), wg.randomNormalFloat32Array(n, 5), np.zeros(n, np.float32)
+        out.append(wg.strsm(dev, "left", "lower", "no-transpose", "non-unit", n, 40, 1.0, tri, n, rhs, 40)["B"])
+        out.append(wg.sgemv(dev, "no-transpose", n, n, 1.0, tri, n, x, 1, 0.0, y, 1)["y"])
+        return out
+
+    try:
+        dev.set_stream(None)
+        own = results()
+        dev.set_stream(0)
+        default = results()
+    finally:
+        dev.set_stream(None)
+    for i, (a, b) in enumerate(zip(own, default)):
+        assert np.abs(a).max() > 0 and np.array_equal(a, b), i
