@@ -30,6 +30,20 @@ def test_parts_are_joined_at_cluster_scope():
     assert arrivals == ["mbar_arrive_cluster"], arrivals
 
 
+def test_a_pairs_accumulators_change_hands_at_cluster_scope():
+    """TMEM reads are done when tcgen05.wait::ld returns and are ordered by the tcgen05 fences: the
+    arrival releases no memory, but it and the wait must reach the other CTA."""
+    text = source("grouped_common.cuh")
+    arrive = text[text.index("void leader_arrive("):]
+    assert "mbarrier.arrive.relaxed.cluster.shared::cluster.b64" in arrive[:arrive.index("\n}\n")]
+    wait = text[text.index("bool leader_wait("):]
+    assert "if constexpr (CG == 2) return wgtc::mbar_wait_bounded_cluster(" in wait[:wait.index("\n}\n")]
+    for name in ("grouped.cu", "mx.cu"):
+        waits = re.findall(r"(\w+(?:<CG>)?)\(&acc_empty\[b\], ", source(name))
+        assert [w for w in waits if w != "mbar_init"] == ["leader_wait<CG>"], (name, waits)
+        assert source(name).count("leader_arrive<CG>(&acc_empty[b])") == 1
+
+
 def test_the_helpers_name_the_scope():
     text = source("tcgen05.cuh")
     assert "mbarrier.arrive.release.cluster.shared::cluster.b64" in text

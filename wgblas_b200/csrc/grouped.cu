@@ -398,7 +398,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
           const int b = used & 1, kb1 = min(x.k_hi, kb0 + segment);
           const bool end = x.end && kb1 == x.k_hi;
           const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
-          ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u, WAIT_BUDGET));
+          ok = __all_sync(0xffffffffu, wgg::leader_wait<CG>(&acc_empty[b], ((uint32_t)(used >> 1) & 1u) ^ 1u));
           wgtc::tc_fence_after();
           for (int kb = kb0; kb < kb1 && ok; kb++, ring.next()) {
             ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&full[ring.s], ring.round, WAIT_BUDGET));

@@ -326,15 +326,22 @@ __device__ __forceinline__ void cluster_sync() {
   if constexpr (N > 1) wgtc::cluster_sync();
   else __syncthreads();
 }
-// One arrival on the leader's copy of `bar`. What it signals for a pair is that
-// TMEM has been read (ordered by tcgen05.wait and the fences), so it needs no
-// release at cluster scope, which costs about a thousand clocks.
+// One arrival on the leader's copy of `bar`, and the leader's wait for them. What they
+// signal for a pair is that TMEM has been read: tcgen05.wait::ld returned and the
+// tcgen05 fences order it, so the arrival is relaxed, at the scope of both CTAs (a release
+// there waits for the warp's own stores, about a thousand clocks).
 template <int CG>
 __device__ __forceinline__ void leader_arrive(uint64_t *bar) {
   if constexpr (CG == 2)
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(wgtc::mapa_shared(wgtc::smem_addr(bar), 0))
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                     wgtc::mapa_shared(wgtc::smem_addr(bar), 0))
                  : "memory");
   else mbar_arrive(bar);
+}
+template <int CG>
+__device__ __forceinline__ bool leader_wait(uint64_t *bar, uint32_t parity) {
+  if constexpr (CG == 2) return wgtc::mbar_wait_bounded_cluster(bar, parity, WAIT_BUDGET);
+  else return wgtc::mbar_wait_bounded(bar, parity, WAIT_BUDGET);
 }
 // `bar` of every CTA of the pair receives one arrival when the MMAs issued so far complete.
 template <int CG>

@@ -767,7 +767,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_l, const __grid_constant_
         for (int kb0 = x.k_lo; kb0 < x.k_hi && ok; kb0 += segment, used++) {
           const int b = used % S::ACCS, kb1 = min(x.k_hi, kb0 + segment);
           const uint32_t d_tmem = tmem + (uint32_t)(b * S::BN);
-          ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&acc_empty[b], ((uint32_t)(used / S::ACCS) & 1u) ^ 1u, WAIT_BUDGET));
+          ok = __all_sync(0xffffffffu, wgg::leader_wait<CG>(&acc_empty[b], ((uint32_t)(used / S::ACCS) & 1u) ^ 1u));
           wgtc::tc_fence_after();
           for (int kb = kb0; kb < kb1 && ok; kb++, ring.next(), set ^= 1u) {
             ok = __all_sync(0xffffffffu, wgtc::mbar_wait_bounded(&full[ring.s], ring.round, WAIT_BUDGET));
